@@ -1,0 +1,272 @@
+// Microscaled rows (microscaled.h): made from numbers, read back, laid out from a checkpoint's codes, and made by the norm between two sub-layers.
+#include "microscaled.h"
+
+namespace alofa {
+
+// Eight numbers of a row from column c0 on, zeros behind the last column. kVec: rows and row starts are 16-byte aligned and k is a multiple of 8.
+template <typename T, bool kVec>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int c0, int k, float (&v)[8]) {
+  if constexpr (kVec && sizeof(T) == 4) {
+    const float4 a = c0 < k ? *reinterpret_cast<const float4*>(row + c0) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 b = c0 < k ? *reinterpret_cast<const float4*>(row + c0 + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else if constexpr (kVec) {
+    const uint4 a = c0 < k ? *reinterpret_cast<const uint4*>(row + c0) : make_uint4(0, 0, 0, 0);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[2 * e] = __uint_as_float(w[e] << 16), v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c0 + e < k ? load_f32(row + c0 + e) : 0.f;
+  }
+}
+
+// Eight numbers of a block whose three other eights are in the neighbouring lanes, to memory
+template <int kKind>
+__device__ __forceinline__ void put8(uint8_t* __restrict__ out, int64_t scales_at, int64_t r, int c, int k_tiles, const float (&v)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = max(top, mx_magnitude(v[e]));
+  const uint32_t code = mx_scale_of<kKind>(quad_max(top));
+  uint32_t q[2];
+  mx_pack8<kKind>(v, code, q);
+  uint8_t* at = out + mx_place8<kKind>(r, c, k_tiles);
+  if constexpr (kKind == kE2M1) *reinterpret_cast<uint32_t*>(at) = q[0];
+  else *reinterpret_cast<uint2*>(at) = make_uint2(q[0], q[1]);
+  if (c % 4 == 0) out[scales_at + mx_scale_place(r, c / 4, k_tiles)] = static_cast<uint8_t>(code);
+}
+
+// ---- numbers to microscaled rows ---------------------------------------------
+// A thread takes eight numbers of one row; four neighbours make a block.
+template <typename T, int kKind, bool kVec>
+__global__ void __launch_bounds__(256) mx_quantize_kernel(uint8_t* __restrict__ out, int64_t scales_at, const T* __restrict__ x, int64_t ldx, int rows, int k, int k_tiles) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int per_row = 16 * k_tiles;
+  const int64_t r = i / per_row;
+  const int c = static_cast<int>(i % per_row);
+  if (r >= rows) return;      // (a row's threads are a multiple of four)
+  float v[8];
+  load8<T, kVec>(x + r * ldx, 8 * c, k, v);
+  put8<kKind>(out, scales_at, r, c, k_tiles, v);
+}
+
+// ---- the values that microscaled rows stand for --------------------------------
+__device__ __forceinline__ float mx_scaled(float element, uint32_t code) { return code == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(element, static_cast<int>(code) - 127); }
+
+template <typename T, int kKind>
+__global__ void __launch_bounds__(256) mx_values_kernel(T* __restrict__ out, int64_t ldo, const uint8_t* __restrict__ q, int64_t scales_at, int rows, int k, int k_tiles) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int per_row = 16 * k_tiles;
+  const int64_t r = i / per_row;
+  const int c = static_cast<int>(i % per_row);
+  if (r >= rows || 8 * c >= k) return;
+  const uint32_t code = q[scales_at + mx_scale_place(r, c / 4, k_tiles)];
+  const uint8_t* at = q + mx_place8<kKind>(r, c, k_tiles);
+  float v[8];
+  if constexpr (kKind == kE2M1) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(at);
+    const f32x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1);
+    const f32x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
+    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = d[0], v[5] = d[1], v[6] = e[0], v[7] = e[1];
+  } else {
+    const uint2 w = *reinterpret_cast<const uint2*>(at);
+    const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, true);
+    const f32x2_t d = __builtin_amdgcn_cvt_pk_f32_fp8(w.y, false), e = __builtin_amdgcn_cvt_pk_f32_fp8(w.y, true);
+    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = d[0], v[5] = d[1], v[6] = e[0], v[7] = e[1];
+  }
+  T* to = out + r * ldo + 8 * c;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (8 * c + e < k) store_f32(to + e, mx_scaled(v[e], code));
+}
+
+// ---- a checkpoint's codes, row by row, into the order above --------------------
+// A thread lays out eight elements of a row. What the codes hold behind the last number of a row is not looked at.
+template <int kKind>
+__global__ void __launch_bounds__(256) mx_from_codes_kernel(uint8_t* __restrict__ out, int64_t scales_at, const uint8_t* __restrict__ codes, int64_t ld_codes,
+                                                            const uint8_t* __restrict__ scales, int64_t ld_scales, int rows, int k, int k_tiles) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int per_row = 16 * k_tiles;
+  const int64_t r = i / per_row;
+  const int c = static_cast<int>(i % per_row);
+  if (r >= rows) return;
+  const uint8_t* row = codes + r * ld_codes;
+  uint32_t q[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int at = 8 * c + e;
+    if (at >= k) continue;
+    if constexpr (kKind == kE2M1) q[0] |= ((row[at / 2] >> (at % 2 * 4)) & 15u) << (4 * e);
+    else q[e / 4] |= static_cast<uint32_t>(row[at]) << (e % 4 * 8);
+  }
+  uint8_t* to = out + mx_place8<kKind>(r, c, k_tiles);
+  if constexpr (kKind == kE2M1) *reinterpret_cast<uint32_t*>(to) = q[0];
+  else *reinterpret_cast<uint2*>(to) = make_uint2(q[0], q[1]);
+  if (c % 4 == 0) out[scales_at + mx_scale_place(r, c / 4, k_tiles)] = 8 * c < k ? scales[r * ld_scales + c / 4] : 0;
+}
+
+// ---- the norm between two sub-layers -------------------------------------------
+// y rounded to 24 bits so that a later rounding to fewer (22 at most) is the rounding of y itself: towards zero, and the last bit set where anything was lost
+__device__ __forceinline__ float round_to_odd(double y) {
+  const float f = static_cast<float>(y);
+  const double d = static_cast<double>(f);
+  uint32_t u = __float_as_uint(f);
+  if (d != y) u = (u - (fabs(d) > fabs(y) ? 1u : 0u)) | 1u;
+  return y != y ? f : __uint_as_float(u);
+}
+
+// total = x + (add[0] + add[1] + ..) in float, y = total / sqrt(mean(total^2) + eps) * w in double, y to microscaled rows. A block takes a row. The squares' sum and
+// y are in double so that no element depends on the order of a sum: a value next to the middle of two elements would become one or the other.
+// kGroups > 0: a row of at most 2,048 kGroups numbers stays in registers between the sum and the scaling; 0: any row, read twice.
+template <int kKind, int kGroups, bool kVec>
+__global__ void __launch_bounds__(256) rmsnorm_mx_kernel(uint8_t* __restrict__ out, int64_t scales_at, const float* x, int64_t ldx, const float* __restrict__ add, int shares,
+                                                         int64_t share_stride, int64_t ld_add, float* total, int64_t ld_total, const float* __restrict__ w, float eps, int k, int k_tiles) {
+  __shared__ double scratch[4];
+  const int64_t r = blockIdx.x;
+  const int per_row = 16 * k_tiles;
+  auto take = [&](int c, float (&v)[8]) {
+    load8<float, kVec>(x + r * ldx, 8 * c, k, v);
+    if (shares == 0) return;
+    float sum[8];
+    load8<float, kVec>(add + r * ld_add, 8 * c, k, sum);
+    for (int s = 1; s < shares; ++s) {
+      float part[8];
+      load8<float, kVec>(add + s * share_stride + r * ld_add, 8 * c, k, part);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += part[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += sum[e];
+  };
+  auto keep = [&](int c, const float (&v)[8]) {
+    if (total == nullptr || 8 * c >= k) return;
+    float* to = total + r * ld_total + 8 * c;
+    if constexpr (kVec) {
+      *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (8 * c + e < k) to[e] = v[e];
+    }
+  };
+  auto leave = [&](int c, float (&v)[8], double scale) {
+    float weight[8];
+    load8<float, kVec>(w, 8 * c, k, weight);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = round_to_odd(static_cast<double>(v[e]) * scale * static_cast<double>(weight[e]));
+    put8<kKind>(out, scales_at, r, c, k_tiles, v);
+  };
+  double ss = 0;
+  if constexpr (kGroups > 0) {
+    float v[kGroups][8];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const int c = threadIdx.x + 256 * i;
+      take(c, v[i]);      // (nothing but zeros behind the row's end)
+      keep(c, v[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += static_cast<double>(v[i][e]) * static_cast<double>(v[i][e]);
+    }
+    ss = block_sum<double, 256>(ss, scratch);
+    const double scale = 1.0 / sqrt(ss / static_cast<double>(k) + static_cast<double>(eps));
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const int c = threadIdx.x + 256 * i;
+      if (c < per_row) leave(c, v[i], scale);
+    }
+  } else {
+    for (int c = threadIdx.x; c < per_row; c += 256) {
+      float v[8];
+      take(c, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += static_cast<double>(v[e]) * static_cast<double>(v[e]);
+    }
+    ss = block_sum<double, 256>(ss, scratch);
+    const double scale = 1.0 / sqrt(ss / static_cast<double>(k) + static_cast<double>(eps));
+    for (int c = threadIdx.x; c < per_row; c += 256) {
+      float v[8];
+      take(c, v);      // (`total` may be x itself: a thread reads its numbers again before it writes them)
+      keep(c, v);
+      leave(c, v, scale);
+    }
+  }
+}
+
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+static bool sizes_fit(const char* what, int kind, int64_t rows, int64_t k) {
+  if (kind != kE2M1 && kind != kE4M3) set_error("%s: no such kind of element: %d", what, kind);
+  else if (rows < 1 || k < 1 || rows > INT32_MAX - 16 || k > (1 << 24)) set_error("%s: rows=%lld k=%lld", what, static_cast<long long>(rows), static_cast<long long>(k));
+  else if (mx_tiles(rows * 16 * mx_tiles(k, 128), 256) >= 1 << 24) set_error("%s: more blocks than a launch takes: rows=%lld k=%lld", what, static_cast<long long>(rows), static_cast<long long>(k));
+  else return true;
+  return false;
+}
+
+}  // namespace alofa
+
+using namespace alofa;
+
+extern "C" int alofa_mx_quantize(void* out, int kind, const void* x, int dtype, int64_t ldx, int64_t rows, int64_t k, hipStream_t stream) {
+  if (!sizes_fit("mx_quantize", kind, rows, k)) return 1;
+  ALOFA_REQUIRE(out && x && aligned16(out) && (dtype == kF32 || dtype == kBF16) && ldx >= 0, "mx_quantize: operands do not fit: dtype=%d ldx=%lld", dtype, static_cast<long long>(ldx));
+  const int k_tiles = static_cast<int>(mx_tiles(k, 128));
+  const int64_t at = mx_scales_at(rows, k, kind);
+  const unsigned blocks = static_cast<unsigned>(mx_tiles(rows * 16 * k_tiles, 256));
+  const bool vec = aligned16(x) && k % 8 == 0 && ldx % (dtype == kF32 ? 4 : 8) == 0;
+  const int r = static_cast<int>(rows), n = static_cast<int>(k);
+#define GO(T, KIND, VEC) mx_quantize_kernel<T, KIND, VEC><<<blocks, 256, 0, stream>>>(static_cast<uint8_t*>(out), at, static_cast<const T*>(x), ldx, r, n, k_tiles)
+#define GO_VEC(T, KIND) do { if (vec) GO(T, KIND, true); else GO(T, KIND, false); } while (0)
+  if (dtype == kF32) { if (kind == kE2M1) GO_VEC(float, kE2M1); else GO_VEC(float, kE4M3); }
+  else { if (kind == kE2M1) GO_VEC(bf16_t, kE2M1); else GO_VEC(bf16_t, kE4M3); }
+#undef GO_VEC
+#undef GO
+  return check_launch("mx_quantize");
+}
+
+extern "C" int alofa_mx_values(void* out, int dtype, int64_t ldo, const void* q, int kind, int64_t rows, int64_t k, hipStream_t stream) {
+  if (!sizes_fit("mx_values", kind, rows, k)) return 1;
+  ALOFA_REQUIRE(out && q && aligned16(q) && (dtype == kF32 || dtype == kBF16) && ldo >= 0, "mx_values: operands do not fit: dtype=%d ldo=%lld", dtype, static_cast<long long>(ldo));
+  const int k_tiles = static_cast<int>(mx_tiles(k, 128));
+  const int64_t at = mx_scales_at(rows, k, kind);
+  const unsigned blocks = static_cast<unsigned>(mx_tiles(rows * 16 * k_tiles, 256));
+  const int r = static_cast<int>(rows), n = static_cast<int>(k);
+#define GO(T, KIND) mx_values_kernel<T, KIND><<<blocks, 256, 0, stream>>>(static_cast<T*>(out), ldo, static_cast<const uint8_t*>(q), at, r, n, k_tiles)
+  if (dtype == kF32) { if (kind == kE2M1) GO(float, kE2M1); else GO(float, kE4M3); }
+  else { if (kind == kE2M1) GO(bf16_t, kE2M1); else GO(bf16_t, kE4M3); }
+#undef GO
+  return check_launch("mx_values");
+}
+
+extern "C" int alofa_mx_from_codes(void* out, int kind, const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales, int64_t rows, int64_t k, hipStream_t stream) {
+  if (!sizes_fit("mx_from_codes", kind, rows, k)) return 1;
+  ALOFA_REQUIRE(out && codes && scales && aligned16(out) && ld_codes >= 0 && ld_scales >= 0, "mx_from_codes: operands do not fit");
+  const int k_tiles = static_cast<int>(mx_tiles(k, 128));
+  const int64_t at = mx_scales_at(rows, k, kind);
+  const unsigned blocks = static_cast<unsigned>(mx_tiles(rows * 16 * k_tiles, 256));
+#define GO(KIND) mx_from_codes_kernel<KIND><<<blocks, 256, 0, stream>>>(static_cast<uint8_t*>(out), at, static_cast<const uint8_t*>(codes), ld_codes, static_cast<const uint8_t*>(scales), \
+                                                                        ld_scales, static_cast<int>(rows), static_cast<int>(k), k_tiles)
+  if (kind == kE2M1) GO(kE2M1); else GO(kE4M3);
+#undef GO
+  return check_launch("mx_from_codes");
+}
+
+extern "C" int alofa_rmsnorm_mx(void* out, int kind, const float* x, int64_t ldx, const float* add, int shares, int64_t share_stride, int64_t ld_add, float* total, int64_t ld_total,
+                                const float* w, float eps, int64_t rows, int64_t k, hipStream_t stream) {
+  if (!sizes_fit("rmsnorm_mx", kind, rows, k)) return 1;
+  ALOFA_REQUIRE(out && x && w && aligned16(out) && shares >= 0 && (shares == 0 || add) && (shares == 0 || total) && ldx >= 0 && ld_add >= 0 && share_stride >= 0 && ld_total >= 0 && eps > 0.f,
+                "rmsnorm_mx: operands do not fit: shares=%d eps=%g", shares, static_cast<double>(eps));
+  const int k_tiles = static_cast<int>(mx_tiles(k, 128)), n = static_cast<int>(k);
+  const int64_t at = mx_scales_at(rows, k, kind);
+  const bool vec = k % 8 == 0 && aligned16(x) && ldx % 4 == 0 && aligned16(w) && (shares == 0 || (aligned16(add) && ld_add % 4 == 0 && share_stride % 4 == 0)) && (!total || (aligned16(total) && ld_total % 4 == 0));
+  const int groups = (16 * k_tiles + 255) / 256;
+#define GO(KIND, G, VEC) rmsnorm_mx_kernel<KIND, G, VEC><<<static_cast<unsigned>(rows), 256, 0, stream>>>(static_cast<uint8_t*>(out), at, x, ldx, add, shares, share_stride, ld_add, total, ld_total, w, eps, n, k_tiles)
+#define GO_VEC(KIND, G) do { if (vec) GO(KIND, G, true); else GO(KIND, G, false); } while (0)
+#define GO_GROUPS(KIND) do { if (groups == 1) GO_VEC(KIND, 1); else if (groups == 2) GO_VEC(KIND, 2); else if (groups <= 4) GO_VEC(KIND, 4); else GO_VEC(KIND, 0); } while (0)
+  if (kind == kE2M1) GO_GROUPS(kE2M1); else GO_GROUPS(kE4M3);
+#undef GO_GROUPS
+#undef GO_VEC
+#undef GO
+  return check_launch("rmsnorm_mx");
+}

@@ -2815,3 +2815,180 @@ def maps_decode(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cac
           _I(1), _I(int(keep_first)), _F(softcap or 0.0), *end.arguments(), _I(end.true_d), _stream())
     if floats:
         combine_maps(out, sums, heads, d, end, rows=rows)
+
+
+# ------------------------------------------------------------- microscaled rows
+
+MX_KINDS = {"e4m3": 0, "e2m1": 4}      # (as csrc/microscaled.h numbers them)
+MX_BLOCK = 32                          # numbers that share a scale
+
+
+class MXRows:
+    """``rows`` x ``k`` numbers in blocks of 32 along a row: elements of 4 bits (``kind`` "e2m1") or 8 ("e4m3") times a power of two per block, in the order in which the
+    matrix cores take them (csrc/microscaled.h). A matrix [out_features, in_features] that a product reads is such rows of "e2m1". ``buffer``: contiguous uint8 on the
+    GPU of at least ``MXRows.bytes(rows, k, kind)``, 16-byte aligned, that they are to lie in; without it, it is allocated. What it holds is made by ``mx_quantize``,
+    ``mx_from_codes``, ``rmsnorm_mx`` or ``gemm_swiglu_mx``; rows' places follow from all three sizes, so that a buffer is read as what it was made as."""
+    __slots__ = ("rows", "k", "kind", "buffer")
+
+    def __init__(self, rows: int, k: int, kind: str, device=None, buffer: Optional[torch.Tensor] = None):
+        need = self.bytes(rows, k, kind)
+        if buffer is None:
+            buffer = torch.empty(need, dtype=torch.uint8, device=device)
+        _contig("buffer", _gpu("buffer", buffer, torch.uint8, 1))
+        if buffer.numel() < need or buffer.data_ptr() % 16:
+            raise AlofaError("shape_mismatch", "microscaled rows need a 16-byte aligned buffer that holds them", f"bytes={buffer.numel()} wants={need} address={buffer.data_ptr():#x}")
+        self.rows, self.k, self.kind, self.buffer = int(rows), int(k), kind, buffer
+
+    @staticmethod
+    def bytes(rows: int, k: int, kind: str) -> int:
+        """Bytes of device memory for so many rows (filled up to 16) of so many numbers (filled up to 128)."""
+        if kind not in MX_KINDS:
+            raise AlofaError("unsupported", "no such kind of microscaled element", f"kind={kind} known={','.join(MX_KINDS)}")
+        if operator.index(rows) < 1 or operator.index(k) < 1:
+            raise AlofaError("shape_mismatch", "microscaled rows need a row and a number at least", f"rows={rows} k={k}")
+        tiles = (rows + 15) // 16 * ((k + 127) // 128)
+        return tiles * ((1024 if kind == "e2m1" else 2048) + 64)
+
+    def __repr__(self):
+        return f"MXRows({self.rows} x {self.k} {self.kind})"
+
+
+def _mx(name: str, q, kind: Optional[str] = None) -> int:
+    """The number of the kind of microscaled rows; ``kind``: the one they must be of."""
+    if not isinstance(q, MXRows):
+        raise AlofaError("invalid_argument", "kernel operand must be microscaled rows", f"operand={name} type={type(q).__name__}")
+    if kind is not None and q.kind != kind:
+        raise AlofaError("unsupported", "microscaled rows are of the wrong kind", f"operand={name} has={q.kind} wants={kind}")
+    return MX_KINDS[q.kind]
+
+
+def _out_rows(name: str, t: torch.Tensor) -> int:
+    """``_rows`` of a tensor that is written: its rows may not overlap."""
+    ld = _rows(name, t)
+    if t.shape[0] > 1 and ld < t.shape[1]:
+        raise AlofaError("shape_mismatch", "rows that are written may not overlap", f"operand={name} shape={tuple(t.shape)} strides={t.stride()}")
+    return ld
+
+
+def _one_device(*operands) -> None:
+    """The kernels go to the current device's stream: operands of another device are refused."""
+    here = torch.cuda.current_device()
+    for t in operands:
+        if t is not None and t.device.index != here:
+            raise AlofaError("invalid_argument", "kernel operand is not on the current device", f"device={t.device} current={here}")
+
+
+def mx_quantize(out: MXRows, x: torch.Tensor) -> None:
+    """The nearest microscaled rows to ``x`` [rows, k] (float32 or bfloat16, rows contiguous). A block's scale is the smallest power of two under which its largest magnitude is at
+    most half a step beyond the largest element (7 for e2m1, 464 for e4m3), 2^-127 at least; its elements are rounded to the nearest, ties to even. A block with an infinity or a NaN is NaN throughout."""
+    kind = _mx("out", out)
+    _gpu("x", x, None, 2)
+    if tuple(x.shape) != (out.rows, out.k):
+        raise AlofaError("shape_mismatch", "rows to quantise do not fit", f"x={tuple(x.shape)} out={out}")
+    code, ld = dtype_code(x), _rows("x", x)
+    _one_device(out.buffer, x)
+    _call("alofa_mx_quantize", out.buffer, kind, x, code, ld, out.rows, out.k, _stream())
+
+
+def mx_values(out: torch.Tensor, q: MXRows) -> None:
+    """out [rows, k] (float32, or bfloat16 rounded to the nearest) = the values that ``q`` stands for."""
+    kind = _mx("q", q)
+    _gpu("out", out, None, 2)
+    if tuple(out.shape) != (q.rows, q.k):
+        raise AlofaError("shape_mismatch", "values do not fit", f"out={tuple(out.shape)} q={q}")
+    code, ld = dtype_code(out), _out_rows("out", out)
+    _one_device(q.buffer, out)
+    _call("alofa_mx_values", out, code, ld, q.buffer, kind, q.rows, q.k, _stream())
+
+
+def mx_from_codes(codes: torch.Tensor, scales: torch.Tensor, k: int, kind: str = "e2m1", out: Optional[MXRows] = None) -> MXRows:
+    """Microscaled rows from what a checkpoint holds, row by row (both uint8 with contiguous rows): ``codes`` [rows, k] of e4m3, or [rows, ceil(k / 2)] of e2m1, two to a byte, the first in
+    the low half; ``scales`` [rows, ceil(k / 32)], e + 127 for 2^e and 255 for a block that is NaN."""
+    _gpu("codes", codes, torch.uint8, 2), _gpu("scales", scales, torch.uint8, 2)
+    rows = codes.shape[0]
+    if out is None:
+        out = MXRows(rows, k, kind, codes.device)
+    number = _mx("out", out, kind)
+    width = (k + 1) // 2 if kind == "e2m1" else k
+    if tuple(codes.shape) != (rows, width) or tuple(scales.shape) != (rows, (k + MX_BLOCK - 1) // MX_BLOCK) or (out.rows, out.k) != (rows, k):
+        raise AlofaError("shape_mismatch", "codes and scales do not fit", f"codes={tuple(codes.shape)} scales={tuple(scales.shape)} k={k} out={out}")
+    ldc, lds = _rows("codes", codes), _rows("scales", scales)
+    _one_device(out.buffer, codes, scales)
+    _call("alofa_mx_from_codes", out.buffer, number, codes, ldc, scales, lds, rows, k, _stream())
+    return out
+
+
+def rmsnorm_mx(out: MXRows, x: torch.Tensor, w: torch.Tensor, eps: float, add: Optional[torch.Tensor] = None, total: Optional[torch.Tensor] = None) -> None:
+    """out = rmsnorm(total) * w as microscaled rows, total = x + (add[0] + add[1] + ..) added in float32 in that order. ``x`` [T, h] float32; ``add`` [T, h] or [shares, T, h] float32 (a product's sum, or
+    the shares of one: ``gemm_mx_shares``); ``total`` [T, h] float32 receives the sum and may be ``x`` itself (no other overlap); it goes with ``add``. The squares' sum and the scaling are in float64, so that a row's elements do
+    not depend on anything but the row."""
+    kind = _mx("out", out)
+    _gpu("x", x, torch.float32, 2), _contig("w", _gpu("w", w, torch.float32, 1))
+    if tuple(x.shape) != (out.rows, out.k) or w.shape[0] != out.k:
+        raise AlofaError("shape_mismatch", "norm width or rows do not fit", f"out={out} x={tuple(x.shape)} w={tuple(w.shape)}")
+    if not eps > 0:
+        raise AlofaError("invalid_argument", "the norm needs a positive eps", f"eps={eps}")
+    if (add is None) != (total is None):
+        raise AlofaError("invalid_argument", "what is added to the stream and the place of the sum go together")
+    shares, stride, ld_add, ld_total = 0, 0, 0, 0
+    if add is not None:
+        _gpu("add", add, torch.float32), _gpu("total", total, torch.float32, 2)
+        if add.dim() == 2:
+            add = add.unsqueeze(0)
+        if add.dim() != 3 or add.shape[0] < 1 or tuple(add.shape[1:]) != tuple(x.shape) or tuple(total.shape) != tuple(x.shape):
+            raise AlofaError("shape_mismatch", "what is added to the stream does not fit it", f"x={tuple(x.shape)} add={tuple(add.shape)} total={tuple(total.shape)}")
+        shares, stride, ld_add, ld_total = add.shape[0], add.stride(0), _rows("add", add[0]), _out_rows("total", total)
+    ldx = _rows("x", x)
+    _one_device(out.buffer, x, w, add, total)
+    _call("alofa_rmsnorm_mx", out.buffer, kind, x, ldx, add, shares, stride, ld_add, total, ld_total, w, _F(eps), out.rows, out.k, _stream())
+
+
+def _mx_product(a, w, matrices: str = "w") -> tuple:
+    kind = _mx("a", a)
+    _mx(matrices, w, "e2m1")
+    if a.k != w.k:
+        raise AlofaError("shape_mismatch", "matrix product shapes do not fit", f"a={a} {matrices}={w}")
+    return kind, a.rows, w.rows, a.k
+
+
+def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor] = None, add_to_out: bool = False) -> None:
+    """out [M, N] = a @ w.T (+ bias), float32 or bfloat16, or out += a @ w.T when ``add_to_out`` (out is then the float32 residual stream). ``a``: microscaled rows of either kind;
+    ``w``: a matrix [N, K] of e2m1. Sums in float32."""
+    kind, M, N, K = _mx_product(a, w)
+    _gpu("out", out, None, 2)
+    if tuple(out.shape) != (M, N):
+        raise AlofaError("shape_mismatch", "matrix product shapes do not fit", f"a={a} w={w} out={tuple(out.shape)}")
+    if bias is not None:
+        _contig("bias", _gpu("bias", bias, torch.float32, 1))
+        if bias.shape[0] != N:
+            raise AlofaError("shape_mismatch", "bias length does not fit", f"bias={tuple(bias.shape)} N={N}")
+    if add_to_out and out.dtype is not torch.float32:
+        raise AlofaError("invalid_argument", "the residual stream is float32", f"out={out.dtype}")
+    if add_to_out and bias is not None:
+        raise AlofaError("unsupported", "a product that adds to the residual stream takes no bias; add the bias in a buffer of its own")
+    code, ldo = dtype_code(out), _out_rows("out", out)
+    _one_device(out, a.buffer, w.buffer, bias)
+    _call("alofa_gemm_mx", out, code, ldo, 1, 0, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, _stream())
+
+
+def gemm_mx_shares(out: torch.Tensor, a: MXRows, w: MXRows) -> None:
+    """out [shares, M, N] float32, contiguous: the product a @ w.T, each share the sum over a part of K; ``rmsnorm_mx(add=out)`` adds them up. At most K / 128 shares, rounded up."""
+    kind, M, N, K = _mx_product(a, w)
+    _contig("out", _gpu("out", out, torch.float32, 3))
+    if tuple(out.shape[1:]) != (M, N) or not 1 <= out.shape[0] <= (K + 127) // 128:
+        raise AlofaError("shape_mismatch", "the shares of a product do not fit", f"a={a} w={w} out={tuple(out.shape)}")
+    _one_device(out, a.buffer, w.buffer)
+    _call("alofa_gemm_mx", out, F32, N, out.shape[0], M * N, a.buffer, kind, w.buffer, None, M, N, K, STORE, _stream())
+
+
+def gemm_swiglu_mx(out: MXRows, a: MXRows, w_gate: MXRows, w_up: MXRows, act: str = "silu") -> None:
+    """out [M, N] = act(a @ w_gate.T) * (a @ w_up.T) as microscaled rows, act "silu" or "gelu_tanh"; the products and the gate in float32."""
+    if act not in GATED:
+        raise AlofaError("unsupported", "no such activation of a gate", f"act={act}")
+    kind, M, N, K = _mx_product(a, w_gate, "w_gate")
+    _mx_product(a, w_up, "w_up")
+    out_kind = _mx("out", out)
+    if w_up.rows != N or (out.rows, out.k) != (M, N):
+        raise AlofaError("shape_mismatch", "gate/up product shapes do not fit", f"a={a} gate={w_gate} up={w_up} out={out}")
+    _one_device(out.buffer, a.buffer, w_gate.buffer, w_up.buffer)
+    _call("alofa_gemm_swiglu_mx", out.buffer, out_kind, a.buffer, kind, w_gate.buffer, w_up.buffer, M, N, K, int(act == "gelu_tanh"), _stream())
