@@ -31,8 +31,10 @@ class Engine:
                  kv_blocks: Optional[int] = None, block_size: int = 16, token_budget: int = 2048, max_chunk: Optional[int] = None,
                  watermark_permille: int = 900, max_wait_ticks: int = 8, seed: int = 1234, device: str = "cuda:0",
                  trace_path=None, share_prefixes: bool = False, model=None, report=None, run_ahead: bool = True,
-                 memory_fraction: Optional[float] = None):
+                 memory_fraction: Optional[float] = None, matrices: str = "stored"):
         """``model``: a (config, Model) pair already on the device, instead of a folder to load.
+        ``matrices``: "stored", or "mxfp4": the layers' matrices are held in 4 bits, a quarter of the memory that bfloat16 takes and that a decode step
+        reads (``load_model``; a ``model`` that is given is as it is).
         ``report``: a callable that receives one line about device memory at start (default:
         standard error when ALOFA_REPORT_MEMORY is set). ``run_ahead``: a tick reads the tokens of the
         tick before only after its own step is launched (``EngineCore``); off, every tick is synchronous.
@@ -46,7 +48,7 @@ class Engine:
         max_chunk = token_budget if max_chunk is None else max_chunk
         from .csrc.build import load
         load()
-        self.config, self.model = model if model is not None else load_model(Path(model_dir), dtype, device)
+        self.config, self.model = model if model is not None else load_model(Path(model_dir), dtype, device, matrices)
         if max_tokens > self.model.spec.max_positions:
             raise AlofaError("out_of_range", "max_tokens passes the model's position bound", f"max_tokens={max_tokens} max_position_embeddings={self.model.spec.max_positions}")
         needs = self.model.cache_needs()

@@ -12,6 +12,7 @@ never a silent fallback. Names the reference has keep their meaning:
 and the engine's own:
 
   ALOFA_DTYPE              bfloat16 | float32                   (bfloat16)
+  ALOFA_MATRICES           stored | mxfp4: the layers' matrices in 4 bits, with bfloat16   (stored)
   ALOFA_PROMPT_IDS         prompts as token ids, "5,17,3;9,2"   (or the first argument)
   ALOFA_PROMPT_FILE        a file of such prompts, one a line   (when neither of the two is given)
   ALOFA_MAX_NEW            tokens to generate per prompt        (16)
@@ -97,6 +98,11 @@ def main(argv=None) -> int:
     dtype = env_str("ALOFA_DTYPE", "bfloat16")
     if dtype not in ("bfloat16", "float32"):
         raise AlofaError("invalid_argument", "ALOFA_DTYPE is bfloat16 or float32", f"ALOFA_DTYPE={dtype}")
+    matrices = env_str("ALOFA_MATRICES", "stored")
+    if matrices not in ("stored", "mxfp4"):
+        raise AlofaError("invalid_argument", "ALOFA_MATRICES is stored or mxfp4", f"ALOFA_MATRICES={matrices}")
+    if matrices == "mxfp4" and dtype == "float32":
+        raise AlofaError("unsupported", "matrices in 4 bits go with bfloat16; float32 is the exact path", f"ALOFA_DTYPE={dtype} ALOFA_MATRICES={matrices}")
     max_new = env_int("ALOFA_MAX_NEW", 16, 1, 32768)
     text = argv[0] if argv else env_str("ALOFA_PROMPT_IDS", "")
     prompt_file = env_str("ALOFA_PROMPT_FILE", "")
@@ -121,7 +127,7 @@ def main(argv=None) -> int:
 
     budget = env_int("ALOFA_TOKEN_BUDGET", 2048, 1, 1 << 20)
     from .api import Engine
-    engine = Engine(weights, dtype=dtype, max_tokens=max_tokens, max_batch=batch, kv_blocks=kv_blocks or None,
+    engine = Engine(weights, dtype=dtype, matrices=matrices, max_tokens=max_tokens, max_batch=batch, kv_blocks=kv_blocks or None,
                     block_size=block, token_budget=budget,
                     max_chunk=env_int("ALOFA_MAX_CHUNK", budget, 1, 1 << 20),
                     watermark_permille=env_int("ALOFA_WATERMARK_PERMILLE", 900, 1, 1000),

@@ -14,6 +14,7 @@ from .config.base import ModelSpec
 from .config.registry import load_config
 from .errors import AlofaError
 from .parts.base import Runtime, build_part, part_class, tensors_of
+from .parts.microscaled import microscaled
 from .parts.streams import StreamRead
 from .weights.loader import load_weights
 
@@ -116,6 +117,7 @@ class Model:
             part = stack.pop()
             for v in vars(part).values():
                 for t in (v if isinstance(v, (list, tuple)) else [v]):
+                    t = t.buffer if isinstance(t, ops.MXRows) else t
                     if isinstance(t, torch.Tensor) and t.is_cuda and t.data_ptr() not in seen:
                         seen.add(t.data_ptr())
                         total += t.numel() * t.element_size()
@@ -212,11 +214,21 @@ def runtime(dtype="bfloat16", device="cuda:0") -> Runtime:
     return Runtime(dev, dtype)
 
 
-def load_model(model_dir, dtype="bfloat16", device="cuda:0"):
+MATRICES = ("stored", "mxfp4")
+
+
+def load_model(model_dir, dtype="bfloat16", device="cuda:0", matrices="stored"):
     """(config, model) of a folder with config.json and model.safetensors; the
-    model class is chosen by config.json through the architecture registry."""
+    model class is chosen by config.json through the architecture registry. ``matrices`` "mxfp4": the layers' matrices
+    are held in 4 bits with a power of two per 32 (parts/microscaled.py)."""
+    if matrices not in MATRICES:
+        raise AlofaError("invalid_argument", "matrices are held as stored or in mxfp4", f"matrices={matrices}")
     cfg = load_config(model_dir)
     spec = cfg.spec()
     check_spec(spec)
+    if matrices == "mxfp4":
+        if DTYPES.get(dtype, dtype) is torch.float32:
+            raise AlofaError("unsupported", "matrices in 4 bits go with bfloat16; float32 is the exact path", f"dtype={dtype} matrices={matrices}")
+        spec = microscaled(spec)
     weights = load_weights(Path(model_dir), expected_tensors(spec))
     return cfg, Model(spec, weights, runtime(dtype, device))

@@ -2971,6 +2971,11 @@ def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor
     _call("alofa_gemm_mx", out, code, ldo, 1, 0, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, _stream())
 
 
+def mx_shares(M: int, N: int, K: int) -> int:
+    """Into how many shares of K the product of so many rows with an [N, K] matrix is best cut where ``rmsnorm_mx`` adds them up."""
+    return 1
+
+
 def gemm_mx_shares(out: torch.Tensor, a: MXRows, w: MXRows) -> None:
     """out [shares, M, N] float32, contiguous: the product a @ w.T, each share the sum over a part of K; ``rmsnorm_mx(add=out)`` adds them up. At most K / 128 shares, rounded up."""
     kind, M, N, K = _mx_product(a, w)

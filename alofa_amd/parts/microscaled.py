@@ -1,0 +1,80 @@
+"""Layers whose matrices are held in 4 bits: a "prenorm" layer of attention and a gated feed-forward (parts/block.py), its seven matrices as microscaled
+rows of e2m1 (blocks of 32 along the inputs, a power of two each), made of the stored ones when the weights are loaded. What the products read is
+microscaled rows of e4m3: the two norms leave them, the activated gate does, and attention's output is brought into them. Everything else is as
+it was: the stream and all sums in float32, queries, keys and values in bfloat16, embedding, norms' weights, biases and head as stored.
+
+a = stream; n0 = q8(norm0(a)); qkv = n0 Wqkv^T + b; o = q8(attention(qkv)); a += o Wo^T; n1 = q8(norm1(a)); a += q8(act(n1 Wg^T) * (n1 Wu^T)) Wd^T
+
+The output product leaves the shares of its sum and the norm behind it adds them to the stream on its way."""
+from __future__ import annotations
+
+import dataclasses
+
+import torch
+
+from .. import ops
+from ..config.base import ModelSpec, PartSpec
+from ..errors import AlofaError
+from .attention import paged_attend
+from .base import register_part
+from .block import PreNormBlock
+
+KIND = "microscaled_prenorm"
+
+
+def microscaled(spec: ModelSpec) -> ModelSpec:
+    """The same model with the matrices of its layers held in 4 bits; refused for layers of other kinds."""
+    layers = []
+    for layer in spec.layers:
+        kinds = {} if layer.block.kind != "prenorm" else {"mixer": layer.part("mixer").kind, "feed_forward": layer.part("feed_forward").kind, "norms": {n.kind for n in layer.part("norms")}}
+        if kinds != {"mixer": "gqa_attention", "feed_forward": "swiglu", "norms": {"rmsnorm"}}:
+            raise AlofaError("unsupported", "matrices in 4 bits are built for layers of attention and a gated feed-forward with a norm in front of each", f"prefix={layer.prefix} block={layer.block.kind}")
+        layers.append(dataclasses.replace(layer, block=PartSpec(KIND, layer.block.params)))
+    return dataclasses.replace(spec, layers=type(spec.layers)(layers))
+
+
+class MicroscaledPreNorm(PreNormBlock):
+    takes_normed = False      # (its norms leave microscaled rows, which no other part gives)
+
+    def __init__(self, layer, weights, rt):
+        if rt.exact:
+            raise AlofaError("unsupported", "matrices in 4 bits go with bfloat16; float32 is the exact path", f"prefix={layer.prefix}")
+        super().__init__(layer, weights, rt)
+        m, f = self.mixer, self.feed_forward
+        self.w_qkv, self.w_o, self.w_gate, self.w_up, self.w_down = map(self._quantised, (m.w_qkv, m.w_o, f.w_gate, f.w_up, f.w_down))
+        m.w_qkv = m.w_o = f.w_gate = f.w_up = f.w_down = None      # (the parts' own forms of the products are not run)
+
+    @staticmethod
+    def _quantised(w: torch.Tensor) -> ops.MXRows:
+        with torch.cuda.device(w.device):
+            q = ops.MXRows(*w.shape, "e2m1", w.device)
+            ops.mx_quantize(q, w)
+        return q
+
+    @staticmethod
+    def _rows(ctx, name: str, rows: int, k: int) -> ops.MXRows:
+        return ops.MXRows(rows, k, "e4m3", buffer=ctx.scratch(name, (ops.MXRows.bytes(rows, k, "e4m3"),), torch.uint8))
+
+    def forward(self, ctx, entry, hidden):
+        (T, h), m, f = hidden.shape, self.mixer, self.feed_forward
+        normed = self._rows(ctx, "mx_normed", T, h)
+        ops.rmsnorm_mx(normed, hidden, *self.norms[0].as_rmsnorm())
+        qkv = ctx.scratch("qkv", (T, m.qkv_width), self.rt.dtype)
+        ops.gemm_mx(qkv, normed, self.w_qkv, m.b_qkv)
+        attn = ctx.scratch("attn", (T, m.heads * m.d), self.rt.dtype)
+        paged_attend(ctx, entry, qkv, attn, m.heads, m.kv_heads, m.d, m.window, m.scale, m.position, self.rt)
+        rows = self._rows(ctx, "mx_attn", T, m.heads * m.d)
+        ops.mx_quantize(rows, attn)
+        if m.b_o is not None:
+            mixed = ctx.scratch("attn_proj", (T, h), torch.float32)
+            ops.gemm_mx(mixed, rows, self.w_o, m.b_o)
+        else:
+            mixed = ctx.scratch("mx_shares", (ops.mx_shares(T, h, rows.k), T, h), torch.float32)
+            ops.gemm_mx_shares(mixed, rows, self.w_o)
+        ops.rmsnorm_mx(normed, hidden, *self.norms[1].as_rmsnorm(), add=mixed, total=hidden)
+        act = self._rows(ctx, "mx_act", T, f.intermediate)
+        ops.gemm_swiglu_mx(act, normed, self.w_gate, self.w_up, f.activation)
+        ops.gemm_mx(hidden, act, self.w_down, add_to_out=True)
+
+
+register_part("block", KIND, MicroscaledPreNorm)

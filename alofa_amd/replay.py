@@ -2,7 +2,7 @@
 logits; it samples nothing. It drives the engine's own model, step function,
 cache and kernels — the ones generation uses.
 
-    bin/trace_run --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N [--blocks N] [--window-blocks N] [--max-requests N]
+    bin/trace_run --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N [--blocks N] [--window-blocks N] [--max-requests N] [--matrices stored|mxfp4]
 
 Steps come on standard input, one JSON object a line:
 
@@ -47,8 +47,8 @@ class Replayer:
     """The replay loop as an object: one ``step`` per input line."""
 
     def __init__(self, model_dir, dtype: str, max_tokens: int, block_size: int = 16, device: str = "cuda:0",
-                 blocks: Optional[int] = None, window_blocks: Optional[int] = None, max_requests: int = 8):
-        """``blocks``: pages of every pool (default: what ``max_tokens`` tokens take); ``window_blocks``: pages of
+                 blocks: Optional[int] = None, window_blocks: Optional[int] = None, max_requests: int = 8, matrices: str = "stored"):
+        """``matrices``: as for ``load_model``; ``blocks``: pages of every pool (default: what ``max_tokens`` tokens take); ``window_blocks``: pages of
         the pools of groups of layers that see a window only, when they are to differ; ``max_requests``: how many
         requests can be live at a time (each has a slot for state of fixed size)."""
         from .csrc.build import load
@@ -57,7 +57,7 @@ class Replayer:
         from .engine.step import StepFunction
         from .model import load_model
 
-        self.config, self.model = load_model(model_dir, dtype, device)
+        self.config, self.model = load_model(model_dir, dtype, device, matrices)
         n_blocks = int(blocks) if blocks is not None else max(1, (int(max_tokens) + block_size - 1) // block_size)
         needs = self.model.cache_needs()
         if window_blocks is not None:
@@ -134,10 +134,11 @@ def main(argv=None) -> int:
     ap.add_argument("--blocks", type=int, default=None, help="pages of the cache pool, instead of what --max-tokens tokens take")
     ap.add_argument("--window-blocks", type=int, default=None, help="pages of the pools of layers that see a window only (default: as the others)")
     ap.add_argument("--max-requests", type=int, default=4, help="requests that can be live at a time (slots for per-request state)")
+    ap.add_argument("--matrices", choices=["stored", "mxfp4"], default="stored", help="mxfp4: the layers' matrices in 4 bits (with bfloat16)")
     args = ap.parse_args(argv)
     out = Path(args.out)
     out.mkdir(parents=True, exist_ok=True)
-    replayer = Replayer(args.model, args.dtype, args.max_tokens, args.block_size, blocks=args.blocks, window_blocks=args.window_blocks, max_requests=args.max_requests)
+    replayer = Replayer(args.model, args.dtype, args.max_tokens, args.block_size, blocks=args.blocks, window_blocks=args.window_blocks, max_requests=args.max_requests, matrices=args.matrices)
     for line in sys.stdin:
         line = line.strip()
         if not line:

@@ -71,3 +71,41 @@ def silu(z):
 
 def gelu_tanh(z):
     return z / 2 * (1 + np.tanh(np.sqrt(2 / np.pi) * (z + 0.044715 * z ** 3)))
+
+
+# ------------------------------------------------------------- a decoder whose matrices are e2m1 and whose products read e4m3
+
+MATRICES = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj", "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj")
+
+
+def matrices_rounded(w, cfg):
+    """The weights with every layer's seven matrices as e2m1."""
+    out = dict(w)
+    for i in range(cfg["L"]):
+        for name in MATRICES:
+            name = f"model.layers.{i}.{name}.weight"
+            out[name] = rounded(w[name].astype(np.float64), "e2m1").astype(np.float32)
+    return out
+
+
+def forward_logits(w, cfg, ids, store=lambda x: x):
+    """As ``plain.model.forward_logits`` with the matrices of ``matrices_rounded`` and what every product of a layer reads as e4m3. ``store``: applied to queries, keys, values, attention's output and the final norm."""
+    from . import model as pm
+    T, F32 = len(ids), np.float32
+    q8 = lambda x: rounded(x.astype(np.float64), "e4m3").astype(F32)      # noqa: E731
+    positions = np.arange(T)
+    cos, sin = pm.rope_table(T, cfg["d"], cfg["theta"])
+    hidden = pm.embed(w["model.embed_tokens.weight"], ids)
+    for i in range(cfg["L"]):
+        p = f"model.layers.{i}."
+        a = p + "self_attn."
+        n = q8(pm.rmsnorm(hidden, w[p + "input_layernorm.weight"], cfg["eps"]))
+        q, k, v = (store(pm.linear(n, w[a + c + "_proj.weight"], w[a + c + "_proj.bias"])) for c in "qkv")
+        q, k = (store(pm.rope_apply(x, cos, sin, positions, cfg["d"])) for x in (q, k))
+        o = q8(store(pm.attention(q, k, v, cfg["H"], cfg["Hkv"], cfg["d"], cfg["windows"][i])))
+        hidden = pm.add(hidden, pm.linear(o, w[a + "o_proj.weight"]))
+        n = q8(pm.rmsnorm(hidden, w[p + "post_attention_layernorm.weight"], cfg["eps"]))
+        act = q8(pm.swiglu(pm.linear(n, w[p + "mlp.gate_proj.weight"]), pm.linear(n, w[p + "mlp.up_proj.weight"])))
+        hidden = pm.add(hidden, pm.linear(act, w[p + "mlp.down_proj.weight"]))
+    y = store(pm.rmsnorm(hidden, w["model.norm.weight"], cfg["eps"]))
+    return pm.linear(y, pm.output_matrix(w, cfg))

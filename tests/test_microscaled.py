@@ -51,3 +51,44 @@ def test_plain_elements_are_torchs():
     want = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
     got = pm.values(codes[None], np.full((1, 8), 127, dtype=np.uint8), 256, "e4m3")[0]
     assert np.array_equal(got, want, equal_nan=True)
+
+
+# ------------------------------------------------------------- the engine's choice of it
+
+def test_only_layers_that_it_is_built_for(tiny_dirs, tugalix_dirs):
+    from alofa_amd.config.registry import load_config
+    from alofa_amd.parts.microscaled import KIND, microscaled
+    spec = load_config(tiny_dirs["A"]).spec()
+    changed = microscaled(spec)
+    assert [layer.block.kind for layer in changed.layers] == [KIND] * len(spec.layers) and changed.order == spec.order
+    assert [layer.parts for layer in changed.layers] == [layer.parts for layer in spec.layers]
+    for d in tugalix_dirs.values():
+        with pytest.raises(AlofaError):
+            microscaled(load_config(d).spec())
+
+
+def test_the_model_reads_the_same_tensors(tiny_dirs):
+    from alofa_amd.config.registry import load_config
+    from alofa_amd.model import expected_tensors
+    from alofa_amd.parts.microscaled import microscaled
+    spec = load_config(tiny_dirs["C"]).spec()
+    assert list(expected_tensors(microscaled(spec)).items()) == list(expected_tensors(spec).items())
+
+
+@pytest.mark.parametrize("dtype,matrices", [("float32", "mxfp4"), ("bfloat16", "mxfp8"), ("bfloat16", "")])
+def test_choices_that_are_refused(tiny_dirs, dtype, matrices):
+    from alofa_amd.model import load_model
+    with pytest.raises(AlofaError) as e:
+        load_model(tiny_dirs["A"], dtype, "cuda:0", matrices)
+    assert "matrices" in str(e.value)
+
+
+@pytest.mark.parametrize("dtype,matrices", [("float32", "mxfp4"), ("bfloat16", "nvfp4")])
+def test_the_command_refuses_them_too(tiny_dirs, monkeypatch, dtype, matrices):
+    from alofa_amd import cli
+    monkeypatch.setenv("ALOFA_WEIGHTS", str(tiny_dirs["A"]))
+    monkeypatch.setenv("ALOFA_DTYPE", dtype)
+    monkeypatch.setenv("ALOFA_MATRICES", matrices)
+    with pytest.raises(AlofaError) as e:
+        cli.main(["5,6"])
+    assert "ALOFA_MATRICES" in str(e.value)
