@@ -1,0 +1,289 @@
+// Products of microscaled rows with microscaled matrices by tiles, for many rows.
+//
+// A block computes 32 NF WN outputs for 32 MF WM rows, a wave NF x MF tiles of 32 x 32 of them (v_mfma_scale_f32_32x32x64_f8f6f4; the matrix is the first operand, so that a lane holds four
+// outputs of one row side by side). Slabs of 128 along K come from memory straight into a ring of S slabs in LDS (global_load_lds); elements and scales lie in memory as the
+// fragments are read, so a slab is whole runs of 1 KB, one per wave and instruction, and 16 lanes' fragments are 256 bytes in a row: nothing is permuted and no banks meet.
+//
+// Operands of the instruction, lane l: row l % 32; e2m1: the 32 numbers from 32 (l / 32) on; e4m3: the sixteen from 16 (l / 32) on and the sixteen from 32 + 16 (l / 32) on; the scale of block
+// l / 32. acc[e] holds the matrix's row 8 (e / 4) + 4 (l / 32) + e % 4 against the activations' row l % 32.
+#include "gemm_mx.h"
+#include "gemm_tiles.h"
+
+namespace alofa {
+
+template <int kAct, int NF_, int MF_, int WN_, int WM_, int S_>
+struct MxTile {
+  static constexpr int NF = NF_, MF = MF_, WN = WN_, WM = WM_, S = S_, kWaves = WN * WM;
+  static constexpr int BN = 32 * NF * WN, BM = 32 * MF * WM;
+  static constexpr int kRowsPieces = BM / 16 * (kAct == kE2M1 ? 1 : 2), kPieces = BN / 16 + kRowsPieces;      // of 1 KB
+  static_assert(kPieces % kWaves == 0 && (BN + BM) % 64 == 0 && (BN + BM) / 64 <= kWaves, "every wave brings as much");
+  static constexpr int kLoads = kPieces / kWaves + 1;                   // a wave's, per slab
+  static constexpr int kScales = kPieces * 1024, kSlab = kScales + kWaves * 256;
+  static_assert(S * kSlab <= 160 * 1024, "the ring fits LDS");
+};
+
+// What a wave multiplies: acc[i][j] of the matrix's i-th 32 rows and the activations' j-th. `gated`: the first half of a wave's 32-row groups is the gate's, the second the same outputs' of up.
+template <int kAct, typename T, bool kGated>
+__device__ __forceinline__ void mx_tile_product(char* ring, const MxMatrix a, const MxMatrix w, const MxMatrix w2, int m_tile, int n_tile, int k_begin, int k_end, int k_tiles, f32x16 (&acc)[T::NF][T::MF]) {
+  constexpr int NF = T::NF, MF = T::MF, S = T::S, kLoads = T::kLoads, kMatrixPieces = T::BN / 16, kHalf = kMatrixPieces / 2;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int wn = wave % T::WN, wm = wave / T::WN;
+
+  // what this wave brings: pieces wave, wave + kWaves, ..; a piece is a run of 1 KB (tiles behind the last of a matrix come from the last; their results are not stored)
+  const uint8_t *const units = w.units, *const up_units = w2.units, *const scales_of = w.scales, *const up_scales = w2.scales;
+  const uint8_t* from[kLoads - 1];
+  int step[kLoads - 1];
+#pragma unroll
+  for (int i = 0; i < kLoads - 1; ++i) {
+    const int p = wave + i * T::kWaves;
+    if (p < kMatrixPieces) {
+      const bool second = kGated && p >= kHalf;
+      const int t = min(n_tile + (second ? p - kHalf : p), w.tiles - 1);
+      from[i] = (second ? up_units : units) + (static_cast<int64_t>(t) * k_tiles + k_begin) * 1024;
+      step[i] = 1024;
+    } else {
+      const int q = p - kMatrixPieces, t = min(m_tile + (kAct == kE2M1 ? q : q / 2), a.tiles - 1);
+      from[i] = a.units + (static_cast<int64_t>(t) * k_tiles + k_begin) * (mx_units(kAct) * 16) + (kAct == kE2M1 ? 0 : q % 2 * 1024);
+      step[i] = mx_units(kAct) * 16;
+    }
+  }
+  // ... and the scales of four tiles, the matrix's first
+  const uint8_t* scales_from;
+  {
+    const int p = min(4 * wave + lane / 16, kMatrixPieces + T::BM / 16 - 1);
+    const uint8_t* base;
+    int t;
+    if (p < kMatrixPieces) {
+      const bool second = kGated && p >= kHalf;
+      t = min(n_tile + (second ? p - kHalf : p), w.tiles - 1);
+      base = second ? up_scales : scales_of;
+    } else {
+      t = min(m_tile + p - kMatrixPieces, a.tiles - 1);
+      base = a.scales;
+    }
+    scales_from = base + (static_cast<int64_t>(t) * k_tiles + k_begin) * 64 + lane % 16 * 4;
+  }
+  // (Written out as instructions: the compiler, which cannot tell the ring's slabs apart, would wait for every load on its way before any read from LDS. M0 holds the LDS address of the
+  // wave's first lane.)
+  const unsigned ring_at = static_cast<unsigned>(reinterpret_cast<uintptr_t>(ring));
+  const unsigned lane_at = lane * 16;
+  auto bring = [&](unsigned slab_at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kLoads - 1; ++i) {
+      const uint64_t run = reinterpret_cast<uint64_t>(from[i]);      // (the wave's own: said to the compiler, which keeps it in vector registers otherwise)
+      const uint64_t base = (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(run >> 32)))) << 32) |
+                            static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(run)));
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                   :: "s"(__builtin_amdgcn_readfirstlane(ring_at + slab_at + (wave + i * T::kWaves) * 1024)), "v"(lane_at), "s"(base), "r"(ring) : "memory", "m0");
+      from[i] += step[i];
+    }
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                 :: "s"(__builtin_amdgcn_readfirstlane(ring_at + slab_at + T::kScales + wave * 256)), "v"(scales_from), "r"(ring) : "memory", "m0");
+    scales_from += 64;
+  };
+
+#pragma unroll
+  for (int i = 0; i < NF; ++i)
+#pragma unroll
+    for (int j = 0; j < MF; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+  // where this lane's fragments lie within a slab
+  const int half = lane / 32, shift = 8 * half, in_tile = lane % 16 * 16;
+  int w_tile[NF], a_tile[MF];
+#pragma unroll
+  for (int i = 0; i < NF; ++i) w_tile[i] = kGated ? (i < NF / 2 ? (wn * (NF / 2) + i) * 2 : kHalf + (wn * (NF / 2) + i - NF / 2) * 2) : (wn * NF + i) * 2;
+#pragma unroll
+  for (int j = 0; j < MF; ++j) a_tile[j] = (wm * MF + j) * 2;
+  const int odd = lane % 32 / 16;
+
+  auto multiply = [&](const char* slab) __attribute__((always_inline)) {
+    const uint32_t* scales = reinterpret_cast<const uint32_t*>(slab + T::kScales) + lane % 32;
+    int ws[NF], as[MF];
+#pragma unroll
+    for (int i = 0; i < NF; ++i) ws[i] = static_cast<int>(scales[w_tile[i] * 16] >> shift);
+#pragma unroll
+    for (int j = 0; j < MF; ++j) as[j] = static_cast<int>(scales[(kMatrixPieces + a_tile[j]) * 16] >> shift);
+    auto step64 = [&](auto number) __attribute__((always_inline)) {
+      constexpr int s = decltype(number)::value;
+      i32x8 wf[NF], af[MF][kAct == kE2M1 ? 1 : 2];
+#pragma unroll
+      for (int i = 0; i < NF; ++i) {
+        const uint4 v = *reinterpret_cast<const uint4*>(slab + (w_tile[i] + odd) * 1024 + (2 * s + half) * 256 + in_tile);
+        wf[i] = {static_cast<int>(v.x), static_cast<int>(v.y), static_cast<int>(v.z), static_cast<int>(v.w), 0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int j = 0; j < MF; ++j) {
+        const char* rows = slab + kMatrixPieces * 1024;
+        if constexpr (kAct == kE2M1) {
+          const uint4 v = *reinterpret_cast<const uint4*>(rows + (a_tile[j] + odd) * 1024 + (2 * s + half) * 256 + in_tile);
+          af[j][0] = {static_cast<int>(v.x), static_cast<int>(v.y), static_cast<int>(v.z), static_cast<int>(v.w), 0, 0, 0, 0};
+        } else {
+          const char* at = rows + (a_tile[j] + odd) * 2048 + (4 * s + half) * 256 + in_tile;
+          const uint4 lo = *reinterpret_cast<const uint4*>(at), hi = *reinterpret_cast<const uint4*>(at + 512);
+          const uint32_t x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            uint32_t large, small;
+            mx_apart(x[e], large, small);
+            af[j][0][e] = static_cast<int>(small), af[j][1][e] = static_cast<int>(large);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < MF; ++j)
+#pragma unroll
+        for (int part = 0; part < (kAct == kE2M1 ? 1 : 2); ++part)
+#pragma unroll
+          for (int i = 0; i < NF; ++i) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[i], af[j][part], acc[i][j], kE2M1, kAct, 2 * s, ws[i], 2 * s, as[j]);
+    };
+    step64(std::integral_constant<int, 0>{});
+    step64(std::integral_constant<int, 1>{});
+  };
+
+  // Slab k + S - 1 is set out once every wave has read slab k - 1, whose place it takes, i.e. behind the barrier of step k. A wave waits for its own loads of slab k (those of the S - 2 behind it
+  // stay on their way) before the barrier; behind the barrier all of the slab is there.
+  unsigned next_at = 0, at = 0;
+  const auto advance = [](unsigned x) { return x == (S - 1) * T::kSlab ? 0u : x + T::kSlab; };
+#pragma unroll
+  for (int p = 0; p < S - 1; ++p)
+    if (k_begin + p < k_end) {
+      bring(next_at);
+      next_at = advance(next_at);
+    }
+  for (int k = k_begin; k < k_end; ++k) {
+    const int behind = k_end - 1 - k;
+    if (behind >= S - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((S - 2) * kLoads) : "memory");
+    else if (S == 4 && behind == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(kLoads) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if (behind >= S - 1) {
+      bring(next_at);
+      next_at = advance(next_at);
+    }
+    multiply(ring + at);
+    at = advance(at);
+  }
+}
+
+template <typename TO, int kAct, typename T>
+__global__ void __launch_bounds__(T::kWaves * 64) mx_tile_kernel(TO* __restrict__ out, int64_t ldo, int64_t share_stride, MxMatrix a, MxMatrix w, const float* __restrict__ bias, int M, int N, int k_tiles, int tiles_m,
+                                                                 int tiles_n, int shares, int epilogue, int vec) {
+  __shared__ __attribute__((aligned(1024))) char ring[T::S * T::kSlab];
+  const TilePlace place = place_tile(blockIdx.x, tiles_m, tiles_n, shares, true);
+  const int k_begin = static_cast<int>(static_cast<int64_t>(k_tiles) * place.share / shares), k_end = static_cast<int>(static_cast<int64_t>(k_tiles) * (place.share + 1) / shares);
+  f32x16 acc[T::NF][T::MF];
+  mx_tile_product<kAct, T, false>(ring, a, w, w, place.bm * (T::BM / 16), place.bn * (T::BN / 16), k_begin, k_end, k_tiles, acc);
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, wn = wave % T::WN, wm = wave / T::WN;
+  out += place.share * share_stride;
+#pragma unroll
+  for (int j = 0; j < T::MF; ++j)
+#pragma unroll
+    for (int i = 0; i < T::NF; ++i) {
+      const int m = place.bm * T::BM + (wm * T::MF + j) * 32 + lane % 32, n = place.bn * T::BN + (wn * T::NF + i) * 32 + 4 * (lane / 32);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        mx_store4(out, ldo, bias, m, n + 8 * q, M, N, f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]}, epilogue, vec != 0);
+    }
+}
+
+// Gate and up, act(gate) * up, to microscaled rows: a lane has half the numbers of a block of 32, the lane 32 further on the other half.
+template <int kAct, int kOut, typename T, bool kGelu>
+__global__ void __launch_bounds__(T::kWaves * 64) mx_tile_gated_kernel(uint8_t* __restrict__ out, int64_t out_scales_at, int out_tiles, MxMatrix a, MxMatrix gate, MxMatrix up, int M, int N, int k_tiles, int tiles_m,
+                                                                       int tiles_n) {
+  __shared__ __attribute__((aligned(1024))) char ring[T::S * T::kSlab];
+  const TilePlace place = place_tile(blockIdx.x, tiles_m, tiles_n, 1, true);
+  f32x16 acc[T::NF][T::MF];
+  mx_tile_product<kAct, T, true>(ring, a, gate, up, place.bm * (T::BM / 16), place.bn * (T::BN / 32), 0, k_tiles, k_tiles, acc);
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, wn = wave % T::WN, wm = wave / T::WN, half = lane / 32;
+#pragma unroll
+  for (int j = 0; j < T::MF; ++j)
+#pragma unroll
+    for (int i = 0; i < T::NF / 2; ++i) {
+      const int m = place.bm * T::BM + (wm * T::MF + j) * 32 + lane % 32, block = place.bn * (T::BN / 64) + wn * (T::NF / 2) + i;
+      float v[16];
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int n = 32 * block + 8 * (e / 4) + 4 * half + e % 4;
+        v[e] = n < N ? gate_of<kGelu>(acc[i][j][e]) * acc[i + T::NF / 2][j][e] : 0.f;
+        top = max(top, mx_magnitude(v[e]));
+      }
+      const auto other = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+      const uint32_t code = mx_scale_of<kOut>(max(static_cast<uint32_t>(other[0]), static_cast<uint32_t>(other[1])));
+      const float lo[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}, hi[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
+      uint32_t x[2], y[2];
+      mx_pack8<kOut>(lo, code, x);
+      mx_pack8<kOut>(hi, code, y);
+      // the lanes exchange what they hold so that each has a run: the lower ones the block's first half, the upper ones its second
+      const int64_t tile = static_cast<int64_t>(m / 16) * out_tiles + block / 4;
+      if constexpr (kOut == kE4M3) {
+        const auto p = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false), q = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+        if (m < M) *reinterpret_cast<uint4*>(out + ((tile * 8 + 2 * (block % 4) + half) * 16 + m % 16) * 16) = make_uint4(p[0], p[1], q[0], q[1]);
+      } else {
+        const auto p = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
+        const uint32_t mine = p[0], its = p[1];      // (four elements of either half, for two runs of eight)
+        if (m < M) *reinterpret_cast<uint2*>(out + ((tile * 4 + block % 4) * 16 + m % 16) * 16 + 8 * half) = make_uint2((mine & 0xffffu) | (its << 16), (mine >> 16) | (its & 0xffff0000u));
+      }
+      if (m < M && half == 0) out[out_scales_at + mx_scale_place(m, block, out_tiles)] = static_cast<uint8_t>(code);
+    }
+}
+
+namespace {
+
+template <typename TO, int kAct, typename T>
+int go(void* out, int64_t ldo, int shares, int64_t share_stride, const MxMatrix& a, const MxMatrix& w, const float* bias, int M, int N, int k_tiles, int epilogue, bool vec, hipStream_t stream) {
+  const int tiles_m = (M + T::BM - 1) / T::BM, tiles_n = (N + T::BN - 1) / T::BN;
+  mx_tile_kernel<TO, kAct, T><<<static_cast<unsigned>(tiles_m) * tiles_n * shares, T::kWaves * 64, 0, stream>>>(static_cast<TO*>(out), ldo, share_stride, a, w, bias, M, N, k_tiles, tiles_m, tiles_n, shares, epilogue, vec);
+  return check_launch("gemm_mx");
+}
+
+template <int kAct, int kOut, typename T>
+int go_gated(uint8_t* out, int64_t at, int out_tiles, const MxMatrix& a, const MxMatrix& gate, const MxMatrix& up, int M, int N, int k_tiles, bool gelu, hipStream_t stream) {
+  const int tiles_m = (M + T::BM - 1) / T::BM, tiles_n = (out_tiles * 128 + T::BN / 2 - 1) / (T::BN / 2);
+  const unsigned blocks = static_cast<unsigned>(tiles_m) * tiles_n;
+  if (gelu) mx_tile_gated_kernel<kAct, kOut, T, true><<<blocks, T::kWaves * 64, 0, stream>>>(out, at, out_tiles, a, gate, up, M, N, k_tiles, tiles_m, tiles_n);
+  else mx_tile_gated_kernel<kAct, kOut, T, false><<<blocks, T::kWaves * 64, 0, stream>>>(out, at, out_tiles, a, gate, up, M, N, k_tiles, tiles_m, tiles_n);
+  return check_launch("gemm_swiglu_mx");
+}
+
+template <int kAct> using Large = MxTile<kAct, 4, 2, 2, 4, kAct == kE2M1 ? 4 : 3>;      // 256 x 256
+template <int kAct> using Middle = MxTile<kAct, 2, 2, 2, 2, 3>;                          // 128 x 128
+template <int kAct> using Small = MxTile<kAct, 2, 1, 1, 2, 4>;                           // 64 x 64
+
+}  // namespace
+
+template <int kAct>
+static int by_form(int form, void* out, int dtype, int64_t ldo, int shares, int64_t share_stride, const MxMatrix& a, const MxMatrix& w, const float* bias, int M, int N, int k_tiles, int epilogue, bool vec,
+                   hipStream_t stream) {
+#define GO(T) (dtype == kF32 ? go<float, kAct, T<kAct>>(out, ldo, shares, share_stride, a, w, bias, M, N, k_tiles, epilogue, vec, stream) \
+                             : go<bf16_t, kAct, T<kAct>>(out, ldo, shares, share_stride, a, w, bias, M, N, k_tiles, epilogue, vec, stream))
+  return form == kMxLarge ? GO(Large) : form == kMxMiddle ? GO(Middle) : GO(Small);
+#undef GO
+}
+
+int launch_mx_tiles(int form, void* out, int dtype, int64_t ldo, int shares, int64_t share_stride, const MxMatrix& a, int a_kind, const MxMatrix& w, const float* bias, int M, int N, int k_tiles, int epilogue,
+                    bool vec, hipStream_t stream) {
+  if (a_kind == kE2M1) return by_form<kE2M1>(form, out, dtype, ldo, shares, share_stride, a, w, bias, M, N, k_tiles, epilogue, vec, stream);
+  return by_form<kE4M3>(form, out, dtype, ldo, shares, share_stride, a, w, bias, M, N, k_tiles, epilogue, vec, stream);
+}
+
+template <int kAct, int kOut>
+static int by_form_gated(int form, uint8_t* out, int64_t at, int out_tiles, const MxMatrix& a, const MxMatrix& gate, const MxMatrix& up, int M, int N, int k_tiles, bool gelu, hipStream_t stream) {
+  if (form == kMxLarge) return go_gated<kAct, kOut, Large<kAct>>(out, at, out_tiles, a, gate, up, M, N, k_tiles, gelu, stream);
+  if (form == kMxMiddle) return go_gated<kAct, kOut, Middle<kAct>>(out, at, out_tiles, a, gate, up, M, N, k_tiles, gelu, stream);
+  return go_gated<kAct, kOut, Small<kAct>>(out, at, out_tiles, a, gate, up, M, N, k_tiles, gelu, stream);
+}
+
+int launch_mx_tiles_gated(int form, uint8_t* out, int out_kind, int64_t out_scales_at, int out_tiles, const MxMatrix& a, int a_kind, const MxMatrix& gate, const MxMatrix& up, int M, int N, int k_tiles, bool gelu,
+                          hipStream_t stream) {
+#define GO(ACT, OUT) by_form_gated<ACT, OUT>(form, out, out_scales_at, out_tiles, a, gate, up, M, N, k_tiles, gelu, stream)
+  if (a_kind == kE2M1) return out_kind == kE2M1 ? GO(kE2M1, kE2M1) : GO(kE2M1, kE4M3);
+  return out_kind == kE2M1 ? GO(kE4M3, kE2M1) : GO(kE4M3, kE4M3);
+#undef GO
+}
+
+}  // namespace alofa

@@ -2943,6 +2943,15 @@ def rmsnorm_mx(out: MXRows, x: torch.Tensor, w: torch.Tensor, eps: float, add: O
     _call("alofa_rmsnorm_mx", out.buffer, kind, x, ldx, add, shares, stride, ld_add, total, ld_total, w, _F(eps), out.rows, out.k, _stream())
 
 
+MX_FORMS = {None: -1, "stream": 0, "tiles256": 1, "tiles128": 2, "tiles64": 3}      # (as csrc/gemm_mx.h numbers them)
+
+
+def _mx_form(kernel: Optional[str]) -> int:
+    if kernel not in MX_FORMS:
+        raise AlofaError("invalid_argument", "no such product kernel for microscaled rows", f"kernel={kernel}")
+    return MX_FORMS[kernel]
+
+
 def _mx_product(a, w, matrices: str = "w") -> tuple:
     kind = _mx("a", a)
     _mx(matrices, w, "e2m1")
@@ -2951,9 +2960,9 @@ def _mx_product(a, w, matrices: str = "w") -> tuple:
     return kind, a.rows, w.rows, a.k
 
 
-def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor] = None, add_to_out: bool = False) -> None:
+def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor] = None, add_to_out: bool = False, kernel: Optional[str] = None) -> None:
     """out [M, N] = a @ w.T (+ bias), float32 or bfloat16, or out += a @ w.T when ``add_to_out`` (out is then the float32 residual stream). ``a``: microscaled rows of either kind;
-    ``w``: a matrix [N, K] of e2m1. Sums in float32."""
+    ``w``: a matrix [N, K] of e2m1. Sums in float32. ``kernel`` names one of ``MX_FORMS`` instead of the rule by sizes (csrc/gemm_mx.hip)."""
     kind, M, N, K = _mx_product(a, w)
     _gpu("out", out, None, 2)
     if tuple(out.shape) != (M, N):
@@ -2968,7 +2977,7 @@ def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor
         raise AlofaError("unsupported", "a product that adds to the residual stream takes no bias; add the bias in a buffer of its own")
     code, ldo = dtype_code(out), _out_rows("out", out)
     _one_device(out, a.buffer, w.buffer, bias)
-    _call("alofa_gemm_mx", out, code, ldo, 1, 0, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, _stream())
+    _call("alofa_gemm_mx", out, code, ldo, 1, 0, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, _mx_form(kernel), _stream())
 
 
 def mx_shares(M: int, N: int, K: int) -> int:
@@ -2976,18 +2985,18 @@ def mx_shares(M: int, N: int, K: int) -> int:
     return 1
 
 
-def gemm_mx_shares(out: torch.Tensor, a: MXRows, w: MXRows) -> None:
+def gemm_mx_shares(out: torch.Tensor, a: MXRows, w: MXRows, kernel: Optional[str] = None) -> None:
     """out [shares, M, N] float32, contiguous: the product a @ w.T, each share the sum over a part of K; ``rmsnorm_mx(add=out)`` adds them up. At most K / 128 shares, rounded up."""
     kind, M, N, K = _mx_product(a, w)
     _contig("out", _gpu("out", out, torch.float32, 3))
     if tuple(out.shape[1:]) != (M, N) or not 1 <= out.shape[0] <= (K + 127) // 128:
         raise AlofaError("shape_mismatch", "the shares of a product do not fit", f"a={a} w={w} out={tuple(out.shape)}")
     _one_device(out, a.buffer, w.buffer)
-    _call("alofa_gemm_mx", out, F32, N, out.shape[0], M * N, a.buffer, kind, w.buffer, None, M, N, K, STORE, _stream())
+    _call("alofa_gemm_mx", out, F32, N, out.shape[0], M * N, a.buffer, kind, w.buffer, None, M, N, K, STORE, _mx_form(kernel), _stream())
 
 
-def gemm_swiglu_mx(out: MXRows, a: MXRows, w_gate: MXRows, w_up: MXRows, act: str = "silu") -> None:
-    """out [M, N] = act(a @ w_gate.T) * (a @ w_up.T) as microscaled rows, act "silu" or "gelu_tanh"; the products and the gate in float32."""
+def gemm_swiglu_mx(out: MXRows, a: MXRows, w_gate: MXRows, w_up: MXRows, act: str = "silu", kernel: Optional[str] = None) -> None:
+    """out [M, N] = act(a @ w_gate.T) * (a @ w_up.T) as microscaled rows, act "silu" or "gelu_tanh"; the products and the gate in float32. ``kernel`` as for ``gemm_mx``."""
     if act not in GATED:
         raise AlofaError("unsupported", "no such activation of a gate", f"act={act}")
     kind, M, N, K = _mx_product(a, w_gate, "w_gate")
@@ -2996,4 +3005,4 @@ def gemm_swiglu_mx(out: MXRows, a: MXRows, w_gate: MXRows, w_up: MXRows, act: st
     if w_up.rows != N or (out.rows, out.k) != (M, N):
         raise AlofaError("shape_mismatch", "gate/up product shapes do not fit", f"a={a} gate={w_gate} up={w_up} out={out}")
     _one_device(out.buffer, a.buffer, w_gate.buffer, w_up.buffer)
-    _call("alofa_gemm_swiglu_mx", out.buffer, out_kind, a.buffer, kind, w_gate.buffer, w_up.buffer, M, N, K, int(act == "gelu_tanh"), _stream())
+    _call("alofa_gemm_swiglu_mx", out.buffer, out_kind, a.buffer, kind, w_gate.buffer, w_up.buffer, M, N, K, int(act == "gelu_tanh"), _mx_form(kernel), _stream())

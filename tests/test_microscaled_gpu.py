@@ -205,6 +205,60 @@ def test_product(M, N, K, kind):
         assert by == 0 or (out._base[:, N:] == 7).all()
 
 
+def check_gated(out, av, gv, uv, act, out_kind):
+    M, N = out.rows, out.k
+    got = read(out)
+    gate, up = av @ gv.T, av @ uv.T
+    f = getattr(pm, "silu" if act == "silu" else act)(gate)
+    y = f * up
+    # the activations' slopes are at most 1.13; exponential, division and product in float32: some ten roundings, those of the exponent weighted with it (|2 c z| below 2^7 here)
+    dy = 1.13 * off_by(av, gv) * (np.abs(up) + off_by(av, uv)) + np.abs(f) * off_by(av, uv) + 2.0 ** -15 * np.abs(y)
+    # a sum that is off may take a block's scale over a border: half a step of the larger one then
+    e = np.maximum(pm.scale_exponents(np.abs(y) + dy, out_kind), pm.scale_exponents(y, out_kind))
+    assert (np.abs(got - y) <= dy + pm.half_step(np.abs(y) + dy, e, out_kind) * (1 + 1e-12)).all()
+    assert (got == pm.rounded(y, out_kind)).mean() > 0.98 or got.size < 64
+    # what the rows are filled up with is zeros: a product over all of them is the product over N
+    ones = made(np.ones((1, N), np.float32), "e2m1")
+    sums = torch.empty(M, 1, device=DEV)
+    ops.gemm_mx(sums, out, ones)
+    one = np.ones((1, N))
+    assert (np.abs(sums.double().cpu().numpy() - got @ one.T) <= off_by(got, one)).all()
+
+
+FORMS = ["stream", "tiles256", "tiles128", "tiles64"]
+
+
+@pytest.mark.parametrize("kernel", FORMS)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (3, 40, 130), (70, 290, 1100), (300, 530, 384), (513, 260, 257)])
+def test_every_kernel_takes_every_product(M, N, K, kind, kernel):
+    a, w, av, wv = operands(M, N, K, kind, M + N + K)
+    want, off = av @ wv.T, off_by(av, wv)
+    for by in (0, 3):
+        out = strided(numbers(M, N, 4, 3), torch.float32, by)
+        ops.gemm_mx(out, a, w, kernel=kernel)
+        assert (np.abs(out.double().cpu().numpy() - want) <= off).all()
+        assert by == 0 or (out._base[:, N:] == 7).all()
+    tiles = -(-K // 128)
+    for shares in {1, min(3, tiles), tiles}:
+        parts = torch.full((shares, M, N), 7.0, device=DEV)
+        ops.gemm_mx_shares(parts, a, w, kernel=kernel)
+        assert (np.abs(parts.double().sum(0).cpu().numpy() - want) <= off).all()
+
+
+@pytest.mark.parametrize("kernel", FORMS)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("out_kind", KINDS)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (3, 40, 130), (70, 290, 300), (300, 530, 384), (513, 130, 257)])
+def test_every_kernel_takes_every_gated_product(M, N, K, out_kind, kind, kernel):
+    a, g, u = numbers(M, K, 1, 1), numbers(N, K, 2, 1) * np.float32(2 / np.sqrt(K)), numbers(N, K, 3, 1) * np.float32(1 / np.sqrt(K))
+    av, gv, uv = pm.rounded(a.astype(np.float64), kind), pm.rounded(g.astype(np.float64), "e2m1"), pm.rounded(u.astype(np.float64), "e2m1")
+    out = ops.MXRows(M, N, out_kind, DEV)
+    out.buffer.fill_(255)
+    ops.gemm_swiglu_mx(out, made(a, kind), made(g, "e2m1"), made(u, "e2m1"), kernel=kernel)
+    check_gated(out, av, gv, uv, "silu", out_kind)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("M,N,K,shares", [(1, 33, 129, 2), (8, 896, 4864, 3), (40, 130, 1000, 8), (130, 512, 2048, 2), (300, 640, 1152, 9)])
 def test_shares_add_up(M, N, K, shares, kind):
@@ -243,22 +297,7 @@ def test_gated(M, N, K, act, out_kind, kind):
     out = ops.MXRows(M, N, out_kind, DEV)
     out.buffer.fill_(255)
     ops.gemm_swiglu_mx(out, made(a, kind), made(g, "e2m1"), made(u, "e2m1"), act)
-    got = read(out)
-    gate, up = av @ gv.T, av @ uv.T
-    f = getattr(pm, "silu" if act == "silu" else act)(gate)
-    y = f * up
-    # the activations' slopes are at most 1.13; exponential, division and product in float32: some ten roundings, those of the exponent weighted with it (|2 c z| below 2^7 here)
-    dy = 1.13 * off_by(av, gv) * (np.abs(up) + off_by(av, uv)) + np.abs(f) * off_by(av, uv) + 2.0 ** -15 * np.abs(y)
-    # a sum that is off may take a block's scale over a border: half a step of the larger one then
-    e = np.maximum(pm.scale_exponents(np.abs(y) + dy, out_kind), pm.scale_exponents(y, out_kind))
-    assert (np.abs(got - y) <= dy + pm.half_step(np.abs(y) + dy, e, out_kind) * (1 + 1e-12)).all()
-    assert (got == pm.rounded(y, out_kind)).mean() > 0.98 or got.size < 64
-    # what the rows are filled up with is zeros: a product over all of them is the product over N
-    ones = made(np.ones((1, N), np.float32), "e2m1")
-    sums = torch.empty(M, 1, device=DEV)
-    ops.gemm_mx(sums, out, ones)
-    one = np.ones((1, N))
-    assert (np.abs(sums.double().cpu().numpy() - got @ one.T) <= off_by(got, one)).all()
+    check_gated(out, av, gv, uv, act, out_kind)
 
 
 # ------------------------------------------------------------- as they are used together
@@ -366,7 +405,8 @@ def test_refusals():
            lambda: ops.gemm_mx(out, made(numbers(4, 65, 1), "e4m3"), w), lambda: ops.gemm_mx(out[:1].expand(4, 32), a, w),
            lambda: ops.gemm_mx_shares(torch.zeros(2, 4, 32, device=DEV), a, w), lambda: ops.gemm_mx_shares(torch.zeros(0, 4, 32, device=DEV), a, w), lambda: ops.gemm_mx_shares(out, a, w),
            lambda: ops.gemm_swiglu_mx(act, a, w, made(numbers(31, 64, 2), "e2m1")), lambda: ops.gemm_swiglu_mx(act, a, w, a), lambda: ops.gemm_swiglu_mx(a, a, w, w),
-           lambda: ops.gemm_swiglu_mx(act, a, w, w, "relu"), lambda: ops.gemm_swiglu_mx(out, a, w, w)]
+           lambda: ops.gemm_swiglu_mx(act, a, w, w, "relu"), lambda: ops.gemm_swiglu_mx(out, a, w, w),
+           lambda: ops.gemm_mx(out, a, w, kernel="rows"), lambda: ops.gemm_mx_shares(torch.zeros(1, 4, 32, device=DEV), a, w, kernel="tiles512"), lambda: ops.gemm_swiglu_mx(act, a, w, w, kernel="tiled")]
     for k, call in enumerate(bad):
         with pytest.raises(AlofaError):
             call()
