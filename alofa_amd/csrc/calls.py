@@ -95,4 +95,4 @@ def _left_to_python(*operands):
     return None
 
 
-norm = caches = turn = attention = _left_to_python
+norm = caches = turn = attention = mx_matrix = mx_norm = _left_to_python

@@ -57,8 +57,8 @@ __device__ __forceinline__ void mx_store4(TO* __restrict__ out, int64_t ldo, con
     if (n + e < N) store_f32(to + e, epilogue == kMxResidual ? load_f32(to + e) + v[e] : v[e]);
 }
 
-// Which kernel: the one that streams the matrix (gemm_mx.hip), or tiles of 256 x 256, 128 x 128 or 64 x 64 (gemm_mx_tiles.hip)
-enum MxForm : int { kMxStream = 0, kMxLarge = 1, kMxMiddle = 2, kMxSmall = 3 };
+// Which kernel: the one that streams the matrix (gemm_mx.hip), or tiles of so many rows by so many columns (gemm_mx_tiles.hip; with a gate: columns of gate and up together)
+enum MxForm : int { kMxStream = 0, kMx256x256 = 1, kMx256x192 = 2, kMx256x160 = 3, kMx256x128 = 4, kMx128x128 = 5, kMx128x64 = 6, kMx64x64 = 7, kMxForms = 8 };
 
 int launch_mx_tiles(int form, void* out, int dtype, int64_t ldo, int shares, int64_t share_stride, const MxMatrix& a, int a_kind, const MxMatrix& w, const float* bias, int M, int N, int k_tiles, int epilogue, bool vec,
                     hipStream_t stream);

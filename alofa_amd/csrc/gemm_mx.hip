@@ -169,11 +169,28 @@ static bool product_fits(const char* what, const void* a, int a_kind, const void
   return ok;
 }
 
-// Which form a product of M rows with so many rows of the matrix (gate and up together) takes.
-static int form_of(int64_t M, int64_t N, int64_t shares) {
+// Tiles, and what a block of them takes: us a slab of 128 where a compute unit has one block, where it has several (each), and besides the slabs. Measured at 64 to 1,024 blocks of 16 and 48 slabs.
+struct MxCost {
+  int form, rows, columns;
+  float alone, each, besides;
+};
+constexpr MxCost kMxRows8[] = {{kMx256x256, 256, 256, 2.58f, 2.58f, 11.f}, {kMx256x192, 256, 192, 2.05f, 2.05f, 9.f},  {kMx256x160, 256, 160, 1.85f, 1.78f, 8.f}, {kMx256x128, 256, 128, 1.48f, 1.44f, 7.5f},
+                               {kMx128x128, 128, 128, 0.86f, 0.71f, 5.8f}, {kMx128x64, 128, 64, 0.60f, 0.44f, 5.f}, {kMx64x64, 64, 64, 0.57f, 0.31f, 5.f}};
+constexpr MxCost kMxRows4[] = {{kMx256x256, 256, 256, 0.99f, 0.99f, 9.5f}, {kMx256x192, 256, 192, 0.82f, 0.83f, 8.5f}, {kMx256x160, 256, 160, 0.72f, 0.74f, 8.f}, {kMx256x128, 256, 128, 0.58f, 0.53f, 7.f},
+                               {kMx128x128, 128, 128, 0.40f, 0.30f, 6.f}, {kMx128x64, 128, 64, 0.27f, 0.17f, 5.f}, {kMx64x64, 64, 64, 0.21f, 0.10f, 5.f}};
+
+// Which form a product of M rows with N rows of a matrix (gate and up together) takes: the matrix streamed for up to 64 rows, the tiles that the figures above foretell to be done first for more
+static int form_of(int64_t M, int64_t N, int k_tiles, int kind, bool gated, int shares) {
   if (M <= 64) return kMxStream;
-  auto tiles = [&](int64_t side) { return mx_tiles(M, side) * mx_tiles(N, side) * shares; };
-  return tiles(256) >= 200 ? kMxLarge : tiles(128) >= 200 ? kMxMiddle : kMxSmall;
+  int best = kMx64x64;
+  float least = 0.f;
+  for (const MxCost& c : kind == kE2M1 ? kMxRows4 : kMxRows8) {
+    if (gated && c.form == kMx256x160) continue;
+    const int64_t blocks = mx_tiles(M, c.rows) * mx_tiles(N, c.columns) * shares, units = compute_units(), each = mx_tiles(blocks, units);
+    const float us = c.besides + 3.f * static_cast<float>(each - 1) + static_cast<float>(mx_tiles(k_tiles, shares)) * fmaxf(c.alone, static_cast<float>(each) * c.each);
+    if (least == 0.f || us < least) best = c.form, least = us;
+  }
+  return best;
 }
 
 }  // namespace alofa
@@ -188,9 +205,9 @@ extern "C" int alofa_gemm_mx(void* out, int dtype, int64_t ldo, int shares, int6
   ALOFA_REQUIRE(shares >= 1 && shares <= mx_tiles(K, 128) && (shares == 1 || (dtype == kF32 && epilogue == kMxStore && !bias)), "gemm_mx: shares=%d K=%lld", shares, static_cast<long long>(K));
   const int k_tiles = static_cast<int>(mx_tiles(K, 128));
   const MxMatrix ma = matrix_of(a, M, K, a_kind), mw = matrix_of(w, N, K, kE2M1);
-  const int vec = reinterpret_cast<uintptr_t>(out) % (dtype == kF32 ? 16 : 8) == 0 && ldo % 4 == 0 && (shares == 1 || share_stride % 4 == 0);
-  ALOFA_REQUIRE(form >= -1 && form <= kMxSmall, "gemm_mx: form=%d", form);
-  if (form < 0) form = form_of(M, N, shares);
+  const int vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ldo % (dtype == kF32 ? 4 : 8) == 0 && (shares == 1 || share_stride % 4 == 0);
+  ALOFA_REQUIRE(form >= -1 && form < kMxForms, "gemm_mx: form=%d", form);
+  if (form < 0) form = form_of(M, N, k_tiles, a_kind, false, shares);
   if (form != kMxStream) return launch_mx_tiles(form, out, dtype, ldo, shares, share_stride, ma, a_kind, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec, stream);
   const int mt = ma.tiles >= 4 ? 4 : ma.tiles >= 2 ? 2 : 1;
   const dim3 grid(mw.tiles, (ma.tiles + mt - 1) / mt, shares);
@@ -210,8 +227,8 @@ extern "C" int alofa_gemm_swiglu_mx(void* out, int out_kind, const void* a, int 
   const int k_tiles = static_cast<int>(mx_tiles(K, 128)), out_tiles = static_cast<int>(mx_tiles(N, 128));
   const MxMatrix ma = matrix_of(a, M, K, a_kind), mg = matrix_of(gate, N, K, kE2M1), mu = matrix_of(up, N, K, kE2M1);
   const int64_t at = mx_scales_at(M, N, out_kind);
-  ALOFA_REQUIRE(form >= -1 && form <= kMxSmall, "gemm_swiglu_mx: form=%d", form);
-  if (form < 0) form = form_of(M, 2 * N, 1);
+  ALOFA_REQUIRE(form >= -1 && form < kMxForms, "gemm_swiglu_mx: form=%d", form);
+  if (form < 0) form = form_of(M, 256 * static_cast<int64_t>(out_tiles), k_tiles, a_kind, true, 1);
   if (form != kMxStream) return launch_mx_tiles_gated(form, static_cast<uint8_t*>(out), out_kind, at, out_tiles, ma, a_kind, mg, mu, static_cast<int>(M), static_cast<int>(N), k_tiles, gelu != 0, stream);
   const int mt = ma.tiles >= 2 ? 2 : 1;
   const dim3 grid(4 * out_tiles, (ma.tiles + mt - 1) / mt);

@@ -16,8 +16,8 @@ struct MxTile {
   static constexpr int NF = NF_, MF = MF_, WN = WN_, WM = WM_, S = S_, kWaves = WN * WM;
   static constexpr int BN = 32 * NF * WN, BM = 32 * MF * WM;
   static constexpr int kRowsPieces = BM / 16 * (kAct == kE2M1 ? 1 : 2), kPieces = BN / 16 + kRowsPieces;      // of 1 KB
-  static_assert(kPieces % kWaves == 0 && (BN + BM) % 64 == 0 && (BN + BM) / 64 <= kWaves, "every wave brings as much");
-  static constexpr int kLoads = kPieces / kWaves + 1;                   // a wave's, per slab
+  static_assert((BN + BM) / 64 <= kWaves, "a wave brings the scales of four tiles at most");
+  static constexpr int kLoads = (kPieces + kWaves - 1) / kWaves + 1;    // a wave's, per slab (a wave with a piece less brings its first one again)
   static constexpr int kScales = kPieces * 1024, kSlab = kScales + kWaves * 256;
   static_assert(S * kSlab <= 160 * 1024, "the ring fits LDS");
 };
@@ -32,10 +32,10 @@ __device__ __forceinline__ void mx_tile_product(char* ring, const MxMatrix a, co
   // what this wave brings: pieces wave, wave + kWaves, ..; a piece is a run of 1 KB (tiles behind the last of a matrix come from the last; their results are not stored)
   const uint8_t *const units = w.units, *const up_units = w2.units, *const scales_of = w.scales, *const up_scales = w2.scales;
   const uint8_t* from[kLoads - 1];
-  int step[kLoads - 1];
+  int step[kLoads - 1], piece[kLoads - 1];
 #pragma unroll
   for (int i = 0; i < kLoads - 1; ++i) {
-    const int p = wave + i * T::kWaves;
+    const int p = piece[i] = wave + i * T::kWaves < T::kPieces ? wave + i * T::kWaves : wave;
     if (p < kMatrixPieces) {
       const bool second = kGated && p >= kHalf;
       const int t = min(n_tile + (second ? p - kHalf : p), w.tiles - 1);
@@ -74,7 +74,7 @@ __device__ __forceinline__ void mx_tile_product(char* ring, const MxMatrix a, co
       const uint64_t base = (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(run >> 32)))) << 32) |
                             static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(run)));
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                   :: "s"(__builtin_amdgcn_readfirstlane(ring_at + slab_at + (wave + i * T::kWaves) * 1024)), "v"(lane_at), "s"(base), "r"(ring) : "memory", "m0");
+                   :: "s"(__builtin_amdgcn_readfirstlane(ring_at + slab_at + piece[i] * 1024)), "v"(lane_at), "s"(base), "r"(ring) : "memory", "m0");
       from[i] += step[i];
     }
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
@@ -154,7 +154,7 @@ __device__ __forceinline__ void mx_tile_product(char* ring, const MxMatrix a, co
     }
   for (int k = k_begin; k < k_end; ++k) {
     const int behind = k_end - 1 - k;
-    if (behind >= S - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((S - 2) * kLoads) : "memory");
+    if (S > 2 && behind >= S - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((S - 2) * kLoads) : "memory");
     else if (S == 4 && behind == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(kLoads) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -169,6 +169,66 @@ __device__ __forceinline__ void mx_tile_product(char* ring, const MxMatrix a, co
   }
 }
 
+// A wave's tiles on their way out, by way of LDS (`room`: the wave's own): a lane holds four outputs of one row, and rows leave in runs of up to 256 bytes. G: 32-row groups of the matrix at a time.
+template <typename TO>
+constexpr int kGroups = sizeof(TO) == 4 ? 2 : 4;
+template <typename TO>
+constexpr int kRoom = 32 * (kGroups<TO> * 32 * static_cast<int>(sizeof(TO)) + 16);
+
+template <typename TO, int G>
+__device__ __forceinline__ void mx_tile_rows(const f32x16* const (&acc)[G], char* room, TO* __restrict__ out, int64_t ldo, const float* __restrict__ bias, int m0, int n0, int M, int N, int epilogue, bool vec, int lane) {
+  constexpr int kRow = G * 32 * static_cast<int>(sizeof(TO)) + 16, kEach = 16 / static_cast<int>(sizeof(TO)), kLanes = G * 32 / kEach;      // bytes of a row; numbers of a lane; lanes of a row
+  constexpr int kAtOnce = 64 / kLanes, kTimes = 32 / kAtOnce;
+  if (n0 >= N || m0 >= M) return;      // (uniform over the wave)
+  wave_lds_sync();      // (what was there before has been read)
+#pragma unroll
+  for (int i = 0; i < G; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      char* at = room + (lane % 32) * kRow + (32 * i + 8 * q + 4 * (lane / 32)) * static_cast<int>(sizeof(TO));
+      const float v[4] = {(*acc[i])[4 * q], (*acc[i])[4 * q + 1], (*acc[i])[4 * q + 2], (*acc[i])[4 * q + 3]};
+      float b[4] = {0.f, 0.f, 0.f, 0.f};
+      if (bias != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = bias[min(n0 + 32 * i + 8 * q + 4 * (lane / 32) + e, N - 1)];
+      }
+      if constexpr (sizeof(TO) == 4) *reinterpret_cast<float4*>(at) = make_float4(v[0] + b[0], v[1] + b[1], v[2] + b[2], v[3] + b[3]);
+      else *reinterpret_cast<uint2*>(at) = make_uint2(pack_bf16x2(v[0] + b[0], v[1] + b[1]), pack_bf16x2(v[2] + b[2], v[3] + b[3]));
+    }
+  wave_lds_sync();
+  const int r0 = lane / kLanes, n = n0 + lane % kLanes * kEach;
+  const char* from = room + r0 * kRow + lane % kLanes * 16;
+  TO* to = out + static_cast<int64_t>(m0 + r0) * ldo + n;
+  if (vec && n0 + 32 * G <= N && m0 + 32 <= M) {      // (uniform: whole tiles)
+    if constexpr (sizeof(TO) == 4) {
+      if (epilogue == kMxResidual) {
+        float4 old[kTimes];
+#pragma unroll
+        for (int t = 0; t < kTimes; ++t) old[t] = *reinterpret_cast<const float4*>(to + static_cast<int64_t>(t * kAtOnce) * ldo);
+#pragma unroll
+        for (int t = 0; t < kTimes; ++t) {
+          const float4 v = *reinterpret_cast<const float4*>(from + t * kAtOnce * kRow);
+          *reinterpret_cast<float4*>(to + static_cast<int64_t>(t * kAtOnce) * ldo) = make_float4(old[t].x + v.x, old[t].y + v.y, old[t].z + v.z, old[t].w + v.w);
+        }
+        return;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kTimes; ++t) *reinterpret_cast<uint4*>(to + static_cast<int64_t>(t * kAtOnce) * ldo) = *reinterpret_cast<const uint4*>(from + t * kAtOnce * kRow);
+    return;
+  }
+  for (int t = 0; t < kTimes; ++t) {
+    if (m0 + r0 + t * kAtOnce >= M) return;
+    const TO* v = reinterpret_cast<const TO*>(from + t * kAtOnce * kRow);
+    TO* row = to + static_cast<int64_t>(t * kAtOnce) * ldo;
+    for (int e = 0; e < kEach; ++e) {
+      if (n + e >= N) break;
+      if (sizeof(TO) == 4 && epilogue == kMxResidual) store_f32(row + e, load_f32(row + e) + load_f32(v + e));
+      else row[e] = v[e];
+    }
+  }
+}
+
 template <typename TO, int kAct, typename T>
 __global__ void __launch_bounds__(T::kWaves * 64) mx_tile_kernel(TO* __restrict__ out, int64_t ldo, int64_t share_stride, MxMatrix a, MxMatrix w, const float* __restrict__ bias, int M, int N, int k_tiles, int tiles_m,
                                                                  int tiles_n, int shares, int epilogue, int vec) {
@@ -179,15 +239,29 @@ __global__ void __launch_bounds__(T::kWaves * 64) mx_tile_kernel(TO* __restrict_
   mx_tile_product<kAct, T, false>(ring, a, w, w, place.bm * (T::BM / 16), place.bn * (T::BN / 16), k_begin, k_end, k_tiles, acc);
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, wn = wave % T::WN, wm = wave / T::WN;
   out += place.share * share_stride;
+  __syncthreads();      // (the ring is free: nothing is on its way, and every wave has read the last slab)
+  static_assert(T::kWaves * kRoom<TO> <= sizeof(ring), "the rows' way out fits the ring");
+  char* room = ring + wave * kRoom<TO>;
 #pragma unroll
-  for (int j = 0; j < T::MF; ++j)
+  for (int j = 0; j < T::MF; ++j) {
+    const int m0 = place.bm * T::BM + (wm * T::MF + j) * 32, n0 = place.bn * T::BN + wn * T::NF * 32;
+    constexpr int G = kGroups<TO>;
 #pragma unroll
-    for (int i = 0; i < T::NF; ++i) {
-      const int m = place.bm * T::BM + (wm * T::MF + j) * 32 + lane % 32, n = place.bn * T::BN + (wn * T::NF + i) * 32 + 4 * (lane / 32);
+    for (int i = 0; i + G <= T::NF; i += G) {
+      const f32x16* group[G];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        mx_store4(out, ldo, bias, m, n + 8 * q, M, N, f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]}, epilogue, vec != 0);
+      for (int g = 0; g < G; ++g) group[g] = &acc[i + g][j];
+      mx_tile_rows<TO, G>(group, room, out, ldo, bias, m0, n0 + 32 * i, M, N, epilogue, vec != 0, lane);
     }
+    if constexpr (T::NF % G >= 2) {
+      const f32x16* group[2] = {&acc[T::NF / G * G][j], &acc[T::NF / G * G + 1][j]};
+      mx_tile_rows<TO, 2>(group, room, out, ldo, bias, m0, n0 + 32 * (T::NF / G * G), M, N, epilogue, vec != 0, lane);
+    }
+    if constexpr (T::NF % 2 == 1) {
+      const f32x16* group[1] = {&acc[T::NF - 1][j]};
+      mx_tile_rows<TO, 1>(group, room, out, ldo, bias, m0, n0 + 32 * (T::NF - 1), M, N, epilogue, vec != 0, lane);
+    }
+  }
 }
 
 // Gate and up, act(gate) * up, to microscaled rows: a lane has half the numbers of a block of 32, the lane 32 further on the other half.
@@ -204,6 +278,7 @@ __global__ void __launch_bounds__(T::kWaves * 64) mx_tile_gated_kernel(uint8_t* 
 #pragma unroll
     for (int i = 0; i < T::NF / 2; ++i) {
       const int m = place.bm * T::BM + (wm * T::MF + j) * 32 + lane % 32, block = place.bn * (T::BN / 64) + wn * (T::NF / 2) + i;
+      if (block >= 4 * out_tiles) continue;      // (uniform over the wave: columns of the last tile behind what the rows are filled up to)
       float v[16];
       uint32_t top = 0;
 #pragma unroll
@@ -250,32 +325,53 @@ int go_gated(uint8_t* out, int64_t at, int out_tiles, const MxMatrix& a, const M
   return check_launch("gemm_swiglu_mx");
 }
 
-template <int kAct> using Large = MxTile<kAct, 4, 2, 2, 4, kAct == kE2M1 ? 4 : 3>;      // 256 x 256
-template <int kAct> using Middle = MxTile<kAct, 2, 2, 2, 2, 3>;                          // 128 x 128
-template <int kAct> using Small = MxTile<kAct, 2, 1, 1, 2, 4>;                           // 64 x 64
+// Rows by columns of the matrix. A wave of e4m3 has one group of 32 rows, which it takes apart, and as many of the matrix as the tile is wide.
+template <int kAct> using T256x256 = MxTile<kAct, kAct == kE2M1 ? 4 : 8, kAct == kE2M1 ? 2 : 1, kAct == kE2M1 ? 2 : 1, kAct == kE2M1 ? 4 : 8, kAct == kE2M1 ? 4 : 3>;
+template <int kAct> using T256x192 = MxTile<kAct, 6, 1, 1, 8, 3>;
+template <int kAct> using T256x160 = MxTile<kAct, 5, 1, 1, 8, 3>;
+template <int kAct> using T256x128 = MxTile<kAct, 4, 1, 1, 8, 3>;
+template <int kAct> using T128x128 = MxTile<kAct, 4, 1, 1, 4, 3>;
+template <int kAct> using T128x64 = MxTile<kAct, 2, 1, 1, 4, 3>;
+template <int kAct> using T64x64 = MxTile<kAct, 2, 1, 1, 2, 4>;
 
 }  // namespace
 
-template <int kAct>
-static int by_form(int form, void* out, int dtype, int64_t ldo, int shares, int64_t share_stride, const MxMatrix& a, const MxMatrix& w, const float* bias, int M, int N, int k_tiles, int epilogue, bool vec,
-                   hipStream_t stream) {
-#define GO(T) (dtype == kF32 ? go<float, kAct, T<kAct>>(out, ldo, shares, share_stride, a, w, bias, M, N, k_tiles, epilogue, vec, stream) \
-                             : go<bf16_t, kAct, T<kAct>>(out, ldo, shares, share_stride, a, w, bias, M, N, k_tiles, epilogue, vec, stream))
-  return form == kMxLarge ? GO(Large) : form == kMxMiddle ? GO(Middle) : GO(Small);
+template <int kAct, typename TO>
+static int by_form(int form, void* out, int64_t ldo, int shares, int64_t share_stride, const MxMatrix& a, const MxMatrix& w, const float* bias, int M, int N, int k_tiles, int epilogue, bool vec, hipStream_t stream) {
+#define GO(T) return go<TO, kAct, T<kAct>>(out, ldo, shares, share_stride, a, w, bias, M, N, k_tiles, epilogue, vec, stream)
+  switch (form) {
+    case kMx256x256: GO(T256x256);
+    case kMx256x192: GO(T256x192);
+    case kMx256x160: GO(T256x160);
+    case kMx256x128: GO(T256x128);
+    case kMx128x128: GO(T128x128);
+    case kMx128x64: GO(T128x64);
+    default: GO(T64x64);
+  }
 #undef GO
 }
 
 int launch_mx_tiles(int form, void* out, int dtype, int64_t ldo, int shares, int64_t share_stride, const MxMatrix& a, int a_kind, const MxMatrix& w, const float* bias, int M, int N, int k_tiles, int epilogue,
                     bool vec, hipStream_t stream) {
-  if (a_kind == kE2M1) return by_form<kE2M1>(form, out, dtype, ldo, shares, share_stride, a, w, bias, M, N, k_tiles, epilogue, vec, stream);
-  return by_form<kE4M3>(form, out, dtype, ldo, shares, share_stride, a, w, bias, M, N, k_tiles, epilogue, vec, stream);
+#define GO(ACT, TO) by_form<ACT, TO>(form, out, ldo, shares, share_stride, a, w, bias, M, N, k_tiles, epilogue, vec, stream)
+  if (a_kind == kE2M1) return dtype == kF32 ? GO(kE2M1, float) : GO(kE2M1, bf16_t);
+  return dtype == kF32 ? GO(kE4M3, float) : GO(kE4M3, bf16_t);
+#undef GO
 }
 
 template <int kAct, int kOut>
 static int by_form_gated(int form, uint8_t* out, int64_t at, int out_tiles, const MxMatrix& a, const MxMatrix& gate, const MxMatrix& up, int M, int N, int k_tiles, bool gelu, hipStream_t stream) {
-  if (form == kMxLarge) return go_gated<kAct, kOut, Large<kAct>>(out, at, out_tiles, a, gate, up, M, N, k_tiles, gelu, stream);
-  if (form == kMxMiddle) return go_gated<kAct, kOut, Middle<kAct>>(out, at, out_tiles, a, gate, up, M, N, k_tiles, gelu, stream);
-  return go_gated<kAct, kOut, Small<kAct>>(out, at, out_tiles, a, gate, up, M, N, k_tiles, gelu, stream);
+#define GO(T) return go_gated<kAct, kOut, T<kAct>>(out, at, out_tiles, a, gate, up, M, N, k_tiles, gelu, stream)
+  switch (form) {
+    case kMx256x256: GO(T256x256);
+    case kMx256x192: GO(T256x192);
+    case kMx256x128: GO(T256x128);
+    case kMx128x128: GO(T128x128);
+    case kMx128x64: GO(T128x64);
+    case kMx64x64: GO(T64x64);
+    default: set_error("gemm_swiglu_mx: gate and up do not share tiles of this form: %d", form); return 1;
+  }
+#undef GO
 }
 
 int launch_mx_tiles_gated(int form, uint8_t* out, int out_kind, int64_t out_scales_at, int out_tiles, const MxMatrix& a, int a_kind, const MxMatrix& gate, const MxMatrix& up, int M, int N, int k_tiles, bool gelu,

@@ -142,6 +142,48 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return Py_BuildValue("LL", (long long)T, (long long)bs);
 }
 
+// mx_matrix(t, bias or None, rows, columns, device, whether it is written) -> (code, leading dimension): numbers beside microscaled rows, [rows, columns] of that device, and a bias of a float per column
+PyObject* mx_matrix(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6) NOT_HERE;
+  const Tensor* t = gpu(args[0], 2);
+  const int64_t rows = PyLong_AsLongLong(args[2]), columns = PyLong_AsLongLong(args[3]), device = PyLong_AsLongLong(args[4]), written = PyLong_AsLongLong(args[5]);
+  if (PyErr_Occurred()) { PyErr_Clear(); NOT_HERE; }
+  if (!t || t->size(0) != rows || t->size(1) != columns || t->device().index() != device) NOT_HERE;
+  const int code = code_of(*t);
+  const int64_t ld = leading(*t);
+  if ((code != kF32 && code != kBF16) || ld < 0 || (written && rows > 1 && ld < columns)) NOT_HERE;
+  if (args[1] != Py_None) {
+    const Tensor* b = dense(args[1], 1, kF32);
+    if (!b || b->size(0) != columns || b->device().index() != device) NOT_HERE;
+  }
+  return Py_BuildValue("iL", code, (long long)ld);
+}
+
+// mx_norm(x, weight, add or None, total or None, rows, width, device) -> (leading dimension of x, shares, their distance, leading dimension of add, of total)
+PyObject* mx_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7) NOT_HERE;
+  const int64_t rows = PyLong_AsLongLong(args[4]), width = PyLong_AsLongLong(args[5]), device = PyLong_AsLongLong(args[6]);
+  if (PyErr_Occurred()) { PyErr_Clear(); NOT_HERE; }
+  const Tensor *x = gpu(args[0], 2), *w = dense(args[1], 1, kF32);
+  if (!x || !w || code_of(*x) != kF32 || x->size(0) != rows || x->size(1) != width || w->size(0) != width || x->device().index() != device || w->device().index() != device || (args[2] == Py_None) != (args[3] == Py_None)) NOT_HERE;
+  const int64_t ldx = leading(*x);
+  int64_t shares = 0, distance = 0, ld_add = 0, ld_total = 0;
+  if (args[2] != Py_None) {
+    if (!THPVariable_Check(args[2])) NOT_HERE;
+    const Tensor* total = gpu(args[3], 2);
+    const bool flat = THPVariable_Unpack(args[2]).dim() == 2;
+    const Tensor* add = gpu(args[2], flat ? 2 : 3);
+    if (!add || !total || code_of(*add) != kF32 || code_of(*total) != kF32 || add->device().index() != device || total->device().index() != device) NOT_HERE;
+    const int64_t at = flat ? 0 : 1;
+    if (add->size(at) != rows || add->size(at + 1) != width || total->size(0) != rows || total->size(1) != width || (add->stride(at + 1) != 1 && width > 1)) NOT_HERE;
+    shares = flat ? 1 : add->size(0), distance = flat ? 0 : add->stride(0);
+    ld_add = rows > 1 ? add->stride(at) : std::max(add->stride(at), width), ld_total = leading(*total);
+    if (shares < 1 || ld_total < 0 || (rows > 1 && ld_total < width)) NOT_HERE;
+  }
+  if (ldx < 0) NOT_HERE;
+  return Py_BuildValue("LLLLL", (long long)ldx, (long long)shares, (long long)distance, (long long)ld_add, (long long)ld_total);
+}
+
 // call(address, ...): the C entry at that address with a tensor's memory, a number, a float or nothing (a null pointer) for each parameter; its
 // answer. In the calling convention of x86-64 (System V), the only host that this library is built for, integers and pointers travel apart from
 // floats, each kind in its own order whatever the order between them, floats up to the eighth in registers only, and the caller takes its
@@ -323,6 +365,7 @@ PyObject* guarded_call(PyObject* self, PyObject* const* args, Py_ssize_t n) {
 
 #define METHOD(name, function) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(function)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD("product", guarded<product>), METHOD("norm", guarded<norm>), METHOD("caches", guarded<caches>), METHOD("turn", guarded<turn>), METHOD("attention", guarded<attention>),
+                         METHOD("mx_matrix", guarded<mx_matrix>), METHOD("mx_norm", guarded<mx_norm>),
                          METHOD("call", guarded_call<call>), METHOD("note", guarded_call<note>), METHOD("tape", guarded_call<tape>), METHOD("taped", guarded_call<taped>),
                          METHOD("play", guarded_call<play>), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "alofa_fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -77,7 +77,11 @@ _scope = _Scope()      # (a thread's own, as torch's current stream is)
 def _stream() -> int:
     if _scope.stream is not None:
         return _scope.stream
-    return torch.cuda.current_stream().cuda_stream
+    return _current_stream(torch.cuda.current_device())
+
+
+# torch's current stream of a device as the launches take it: its own way to that number where it has one (0.4 us with the device's number; by way of a Stream object 2.7)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 class stream_scope:
@@ -2828,7 +2832,7 @@ class MXRows:
     matrix cores take them (csrc/microscaled.h). A matrix [out_features, in_features] that a product reads is such rows of "e2m1". ``buffer``: contiguous uint8 on the
     GPU of at least ``MXRows.bytes(rows, k, kind)``, 16-byte aligned, that they are to lie in; without it, it is allocated. What it holds is made by ``mx_quantize``,
     ``mx_from_codes``, ``rmsnorm_mx`` or ``gemm_swiglu_mx``; rows' places follow from all three sizes, so that a buffer is read as what it was made as."""
-    __slots__ = ("rows", "k", "kind", "buffer")
+    __slots__ = ("rows", "k", "kind", "buffer", "number", "device")      # (number: the kind's, as csrc/microscaled.h has it; device: its index)
 
     def __init__(self, rows: int, k: int, kind: str, device=None, buffer: Optional[torch.Tensor] = None):
         need = self.bytes(rows, k, kind)
@@ -2837,7 +2841,7 @@ class MXRows:
         _contig("buffer", _gpu("buffer", buffer, torch.uint8, 1))
         if buffer.numel() < need or buffer.data_ptr() % 16:
             raise AlofaError("shape_mismatch", "microscaled rows need a 16-byte aligned buffer that holds them", f"bytes={buffer.numel()} wants={need} address={buffer.data_ptr():#x}")
-        self.rows, self.k, self.kind, self.buffer = int(rows), int(k), kind, buffer
+        self.rows, self.k, self.kind, self.buffer, self.number, self.device = int(rows), int(k), kind, buffer, MX_KINDS[kind], buffer.device.index
 
     @staticmethod
     def bytes(rows: int, k: int, kind: str) -> int:
@@ -2870,9 +2874,12 @@ def _out_rows(name: str, t: torch.Tensor) -> int:
     return ld
 
 
+_here = torch.cuda.current_device      # (the kernels go to the current device's stream)
+
+
 def _one_device(*operands) -> None:
-    """The kernels go to the current device's stream: operands of another device are refused."""
-    here = torch.cuda.current_device()
+    """Operands of another device than the current one are refused."""
+    here = _here()
     for t in operands:
         if t is not None and t.device.index != here:
             raise AlofaError("invalid_argument", "kernel operand is not on the current device", f"device={t.device} current={here}")
@@ -2881,6 +2888,9 @@ def _one_device(*operands) -> None:
 def mx_quantize(out: MXRows, x: torch.Tensor) -> None:
     """The nearest microscaled rows to ``x`` [rows, k] (float32 or bfloat16, rows contiguous). A block's scale is the smallest power of two under which its largest magnitude is at
     most half a step beyond the largest element (7 for e2m1, 464 for e4m3), 2^-127 at least; its elements are rounded to the nearest, ties to even. A block with an infinity or a NaN is NaN throughout."""
+    if type(out) is MXRows and _here() == out.device and (sizes := _native().mx_matrix(x, None, out.rows, out.k, out.device, 0)) is not None:
+        _call("alofa_mx_quantize", out.buffer, out.number, x, *sizes, out.rows, out.k, _stream())
+        return
     kind = _mx("out", out)
     _gpu("x", x, None, 2)
     if tuple(x.shape) != (out.rows, out.k):
@@ -2892,6 +2902,9 @@ def mx_quantize(out: MXRows, x: torch.Tensor) -> None:
 
 def mx_values(out: torch.Tensor, q: MXRows) -> None:
     """out [rows, k] (float32, or bfloat16 rounded to the nearest) = the values that ``q`` stands for."""
+    if type(q) is MXRows and _here() == q.device and (sizes := _native().mx_matrix(out, None, q.rows, q.k, q.device, 1)) is not None:
+        _call("alofa_mx_values", out, *sizes, q.buffer, q.number, q.rows, q.k, _stream())
+        return
     kind = _mx("q", q)
     _gpu("out", out, None, 2)
     if tuple(out.shape) != (q.rows, q.k):
@@ -2922,6 +2935,10 @@ def rmsnorm_mx(out: MXRows, x: torch.Tensor, w: torch.Tensor, eps: float, add: O
     """out = rmsnorm(total) * w as microscaled rows, total = x + (add[0] + add[1] + ..) added in float32 in that order. ``x`` [T, h] float32; ``add`` [T, h] or [shares, T, h] float32 (a product's sum, or
     the shares of one: ``gemm_mx_shares``); ``total`` [T, h] float32 receives the sum and may be ``x`` itself (no other overlap); it goes with ``add``. The squares' sum and the scaling are in float64, so that a row's elements do
     not depend on anything but the row."""
+    if type(out) is MXRows and eps > 0 and _here() == out.device and (sizes := _native().mx_norm(x, w, add, total, out.rows, out.k, out.device)) is not None:
+        ldx, shares, stride, ld_add, ld_total = sizes
+        _call("alofa_rmsnorm_mx", out.buffer, out.number, x, ldx, add, shares, stride, ld_add, total, ld_total, w, _F(eps), out.rows, out.k, _stream())
+        return
     kind = _mx("out", out)
     _gpu("x", x, torch.float32, 2), _contig("w", _gpu("w", w, torch.float32, 1))
     if tuple(x.shape) != (out.rows, out.k) or w.shape[0] != out.k:
@@ -2943,7 +2960,7 @@ def rmsnorm_mx(out: MXRows, x: torch.Tensor, w: torch.Tensor, eps: float, add: O
     _call("alofa_rmsnorm_mx", out.buffer, kind, x, ldx, add, shares, stride, ld_add, total, ld_total, w, _F(eps), out.rows, out.k, _stream())
 
 
-MX_FORMS = {None: -1, "stream": 0, "tiles256": 1, "tiles128": 2, "tiles64": 3}      # (as csrc/gemm_mx.h numbers them)
+MX_FORMS = {None: -1, "stream": 0, "256x256": 1, "256x192": 2, "256x160": 3, "256x128": 4, "128x128": 5, "128x64": 6, "64x64": 7}      # (as csrc/gemm_mx.h numbers them: the streaming kernel, or tiles of rows x columns)
 
 
 def _mx_form(kernel: Optional[str]) -> int:
@@ -2953,6 +2970,8 @@ def _mx_form(kernel: Optional[str]) -> int:
 
 
 def _mx_product(a, w, matrices: str = "w") -> tuple:
+    if type(a) is MXRows and type(w) is MXRows and w.number == 4 and a.k == w.k:
+        return a.number, a.rows, w.rows, a.k
     kind = _mx("a", a)
     _mx(matrices, w, "e2m1")
     if a.k != w.k:
@@ -2964,6 +2983,10 @@ def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor
     """out [M, N] = a @ w.T (+ bias), float32 or bfloat16, or out += a @ w.T when ``add_to_out`` (out is then the float32 residual stream). ``a``: microscaled rows of either kind;
     ``w``: a matrix [N, K] of e2m1. Sums in float32. ``kernel`` names one of ``MX_FORMS`` instead of the rule by sizes (csrc/gemm_mx.hip)."""
     kind, M, N, K = _mx_product(a, w)
+    form = -1 if kernel is None else _mx_form(kernel)
+    if _here() == a.device == w.device and (sizes := _native().mx_matrix(out, bias, M, N, a.device, 1)) is not None and (not add_to_out or (bias is None and sizes[0] == F32)):
+        _call("alofa_gemm_mx", out, *sizes, 1, 0, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, form, _stream())
+        return
     _gpu("out", out, None, 2)
     if tuple(out.shape) != (M, N):
         raise AlofaError("shape_mismatch", "matrix product shapes do not fit", f"a={a} w={w} out={tuple(out.shape)}")
@@ -2977,7 +3000,7 @@ def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor
         raise AlofaError("unsupported", "a product that adds to the residual stream takes no bias; add the bias in a buffer of its own")
     code, ldo = dtype_code(out), _out_rows("out", out)
     _one_device(out, a.buffer, w.buffer, bias)
-    _call("alofa_gemm_mx", out, code, ldo, 1, 0, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, _mx_form(kernel), _stream())
+    _call("alofa_gemm_mx", out, code, ldo, 1, 0, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, form, _stream())
 
 
 def mx_shares(M: int, N: int, K: int) -> int:
