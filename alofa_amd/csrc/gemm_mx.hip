@@ -6,18 +6,20 @@
 // holds its row 4 (l / 16) + e against the activations' row l % 16, four outputs that lie side by side.
 #include "gemm_mx.h"
 
+#include <initializer_list>
+
 namespace alofa {
 
 template <int kKind>
 struct MxFragment {
   uint4 half[kKind == kE2M1 ? 1 : 2];
   uint32_t scale;      // of the row's four blocks
-  __device__ __forceinline__ void load(const MxMatrix& m, int row_tile, int k_tile, int k_tiles, int lane) {
-    const int64_t tile = static_cast<int64_t>(row_tile) * k_tiles + k_tile;
-    const uint4* at = reinterpret_cast<const uint4*>(m.units) + tile * mx_units(kKind) + lane;
-    half[0] = at[0];
-    if constexpr (kKind == kE4M3) half[1] = at[64];
-    scale = reinterpret_cast<const uint32_t*>(m.scales)[tile * 16 + lane % 16];
+  // tile: which of the matrix's; at: the lane's unit of it (its row and group)
+  __device__ __forceinline__ void load(const MxMatrix& m, int64_t tile, int at) {
+    const uint4* from = reinterpret_cast<const uint4*>(m.units) + tile * mx_units(kKind) + at;
+    half[0] = from[0];
+    if constexpr (kKind == kE4M3) half[1] = from[64];
+    scale = reinterpret_cast<const uint32_t*>(m.scales)[tile * 16 + at % 16];
   }
 };
 
@@ -52,61 +54,103 @@ __device__ __forceinline__ f32x4 mx_multiply(const MxOperand<kE2M1>& w, const Mx
 }
 
 // ---- few rows: the matrix is streamed once -------------------------------------
-// A block computes NT tiles of 16 outputs for MT tiles of 16 rows. Its waves share out K tile by tile, every wave with U tiles of 128 on their way; the waves' sums meet in
-// LDS and are added in the waves' order.
+// A block computes NT tiles of 16 outputs for MT tiles of 16 rows. Its waves share out K tile by tile, every wave with two sets of U tiles of 128 on their way or under its products; the waves' sums
+// meet in LDS and are added in the waves' order. Lanes whose row lies behind the last one read the last one again: memory is asked for rows that there are only.
 template <int kAct, int NT, int MT, int kWaves, int U>
-__device__ __forceinline__ void mx_stream(const MxMatrix& a, const MxMatrix (&w)[NT], const int (&w_tile)[NT], int first_m_tile, int k_begin, int k_end, int k_tiles, f32x4 (&acc)[NT][MT]) {
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, shift = 8 * (lane / 16);
-  int a_tile[MT];
+__device__ __forceinline__ void mx_stream(const MxMatrix& a, const MxMatrix (&w)[NT], const int (&w_tile)[NT], int M, int first_m_tile, int k_begin, int k_end, int k_tiles, f32x4 (&acc)[NT][MT]) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, shift = 8 * (lane / 16);
+  int64_t a_tile[MT];
+  int a_at[MT];
 #pragma unroll
-  for (int j = 0; j < MT; ++j) a_tile[j] = min(first_m_tile + j, a.tiles - 1);      // (results of rows behind the last are not stored)
+  for (int j = 0; j < MT; ++j) {
+    const int t = min(first_m_tile + j, a.tiles - 1);
+    a_tile[j] = static_cast<int64_t>(t) * k_tiles;
+    a_at[j] = lane / 16 * 16 + min(lane % 16, M - 1 - 16 * t);
+  }
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int kt = k_begin + wave; kt < k_end; kt += kWaves * U) {
-    MxFragment<kE2M1> fw[U][NT];
-    MxFragment<kAct> fa[U][MT];
+  struct Set {
+    MxFragment<kE2M1> w[U][NT];
+    MxFragment<kAct> a[U][MT];
+  };
+  // (every load is always made, so that the compiler can count them: behind the end of K the last tile again, whose elements of the matrix become zeros)
+  auto load = [&](Set& s, int kt) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int at = min(kt + u * kWaves, k_end - 1);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) fw[u][i].load(w[i], w_tile[i], at, k_tiles, lane);
+      for (int i = 0; i < NT; ++i) s.w[u][i].load(w[i], static_cast<int64_t>(w_tile[i]) * k_tiles + at, lane);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) fa[u][j].load(a, a_tile[j], at, k_tiles, lane);
+      for (int j = 0; j < MT; ++j) s.a[u][j].load(a, a_tile[j] + at, a_at[j]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&](Set& s, int kt) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (kt + u * kWaves >= k_end) break;      // (uniform over the wave)
+      const uint32_t there = kt + u * kWaves < k_end ? ~0u : 0u;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        uint4& x = s.w[u][i].half[0];
+        x = make_uint4(x.x & there, x.y & there, x.z & there, x.w & there);
+      }
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        const MxOperand<kAct> a_op(fa[u][j], shift);
+        const MxOperand<kAct> a_op(s.a[u][j], shift);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) acc[i][j] = mx_multiply<kAct>(MxOperand<kE2M1>(fw[u][i], shift), a_op, acc[i][j]);
+        for (int i = 0; i < NT; ++i) acc[i][j] = mx_multiply<kAct>(MxOperand<kE2M1>(s.w[u][i], shift), a_op, acc[i][j]);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr int kStep = kWaves * U;
+  int kt = k_begin + wave;
+  if (kt >= k_end) return;      // (uniform over the wave)
+  Set s0, s1;
+  load(s0, kt);
+  while (true) {
+    if (kt + kStep >= k_end) {
+      multiply(s0, kt);
+      return;
+    }
+    load(s1, kt + kStep);
+    multiply(s0, kt);
+    kt += 2 * kStep;
+    if (kt >= k_end) {
+      multiply(s1, kt - kStep);
+      return;
+    }
+    load(s0, kt);
+    multiply(s1, kt - kStep);
   }
 }
 
-template <typename TO, int kAct, int MT, int kWaves, int U>
-__global__ void __launch_bounds__(kWaves * kWave) mx_stream_kernel(TO* __restrict__ out, int64_t ldo, int64_t share_stride, MxMatrix a, MxMatrix w, const float* __restrict__ bias, int M, int N,
+template <typename TO, int kAct, int NT, int MT, int kWaves, int U>
+__global__ void __launch_bounds__(kWaves * kWave, MT == 1 ? 4 : 1) mx_stream_kernel(TO* __restrict__ out, int64_t ldo, int64_t share_stride, MxMatrix a, MxMatrix w, const float* __restrict__ bias, int M, int N,
                                                                    int k_tiles, int epilogue, int vec) {
-  __shared__ f32x4 sums[MT][kWaves][kWave];
+  __shared__ f32x4 sums[NT * MT][kWaves][kWave];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const int shares = gridDim.z, share = blockIdx.z;
   const int k_begin = static_cast<int>(static_cast<int64_t>(k_tiles) * share / shares), k_end = static_cast<int>(static_cast<int64_t>(k_tiles) * (share + 1) / shares);
-  const MxMatrix ws[1] = {w};
-  const int tiles[1] = {static_cast<int>(blockIdx.x)};
-  f32x4 acc[1][MT];
-  mx_stream<kAct, 1, MT, kWaves, U>(a, ws, tiles, blockIdx.y * MT, k_begin, k_end, k_tiles, acc);
+  MxMatrix ws[NT];
+  int tiles[NT];
 #pragma unroll
-  for (int j = 0; j < MT; ++j) sums[j][wave][lane] = acc[0][j];
+  for (int i = 0; i < NT; ++i) ws[i] = w, tiles[i] = min(static_cast<int>(blockIdx.x) * NT + i, w.tiles - 1);
+  f32x4 acc[NT][MT];
+  mx_stream<kAct, NT, MT, kWaves, U>(a, ws, tiles, M, blockIdx.y * MT, k_begin, k_end, k_tiles, acc);
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sums[i * MT + j][wave][lane] = acc[i][j];
   __syncthreads();
-  if (wave >= MT) return;
-  f32x4 v = sums[wave][0][lane];
+  for (int f = wave; f < NT * MT; f += kWaves) {
+    f32x4 v = sums[f][0][lane];
 #pragma unroll
-  for (int s = 1; s < kWaves; ++s) v += sums[wave][s][lane];
-  mx_store4(out + share * share_stride, ldo, bias, (blockIdx.y * MT + wave) * 16 + lane % 16, blockIdx.x * 16 + lane / 16 * 4, M, N, v, epilogue, vec != 0);
+    for (int s = 1; s < kWaves; ++s) v += sums[f][s][lane];
+    mx_store4(out + share * share_stride, ldo, bias, (blockIdx.y * MT + f % MT) * 16 + lane % 16, (blockIdx.x * NT + f / MT) * 16 + lane / 16 * 4, M, N, v, epilogue, vec != 0);
+  }
 }
 
 // Gate and up of the same 32 outputs, act(gate) * up, one block of a microscaled row of the output.
@@ -120,7 +164,7 @@ __global__ void __launch_bounds__(kWaves * kWave) mx_stream_gated_kernel(uint8_t
   const int t0 = min(2 * static_cast<int>(blockIdx.x), gate.tiles - 1), t1 = min(2 * static_cast<int>(blockIdx.x) + 1, gate.tiles - 1);
   const int tiles[4] = {t0, t1, t0, t1};
   f32x4 acc[4][MT];
-  mx_stream<kAct, 4, MT, kWaves, U>(a, ws, tiles, blockIdx.y * MT, 0, k_tiles, k_tiles, acc);
+  mx_stream<kAct, 4, MT, kWaves, U>(a, ws, tiles, M, blockIdx.y * MT, 0, k_tiles, k_tiles, acc);
   for (int j = 0; j < MT; ++j) {
     __syncthreads();
 #pragma unroll
@@ -169,55 +213,126 @@ static bool product_fits(const char* what, const void* a, int a_kind, const void
   return ok;
 }
 
-// Tiles, and what a block of them takes: us a slab of 128 where a compute unit has one block, where it has several (each), and besides the slabs. Measured at 64 to 1,024 blocks of 16 and 48 slabs.
+// The shares of a sum added up in their order, on to the epilogue. A thread takes four outputs of a row.
+template <typename TO>
+__global__ void __launch_bounds__(256) mx_sum_kernel(TO* __restrict__ out, int64_t ldo, const float* __restrict__ parts, int shares, const float* __restrict__ bias, int M, int N, int epilogue, int vec) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int quads = (N + 3) / 4;
+  const int m = static_cast<int>(i / quads), n = static_cast<int>(i % quads) * 4;
+  if (m >= M) return;
+  const int64_t share = static_cast<int64_t>(M) * N;
+  const float* at = parts + static_cast<int64_t>(m) * N + n;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < shares; ++s, at += share) {
+    if (N % 4 == 0) {
+      const float4 x = *reinterpret_cast<const float4*>(at);
+      v += f32x4{x.x, x.y, x.z, x.w};
+    } else {
+      for (int e = 0; e < 4; ++e)
+        if (n + e < N) v[e] += at[e];
+    }
+  }
+  mx_store4(out, ldo, bias, m, n, M, N, v, epilogue, vec != 0);
+}
+
+// What a product takes in each form, in us as measured, and how it is chosen. Tiles: a slab of 128 where a compute unit has one block, where it has several (each), and besides the slabs (64 to 1,024 blocks
+// of 16 and 48 slabs). The streaming kernel: a tile of 128 along K of a wave, for one, two and four tiles of rows (and of the matrix). A sum that is shared out over K takes a launch more, which adds the shares up, unless a norm does.
 struct MxCost {
   int form, rows, columns;
   float alone, each, besides;
 };
 constexpr MxCost kMxRows8[] = {{kMx256x256, 256, 256, 2.58f, 2.58f, 11.f}, {kMx256x192, 256, 192, 2.05f, 2.05f, 9.f},  {kMx256x160, 256, 160, 1.85f, 1.78f, 8.f}, {kMx256x128, 256, 128, 1.48f, 1.44f, 7.5f},
-                               {kMx128x128, 128, 128, 0.86f, 0.71f, 5.8f}, {kMx128x64, 128, 64, 0.60f, 0.44f, 5.f}, {kMx64x64, 64, 64, 0.57f, 0.31f, 5.f}};
+                               {kMx128x128, 128, 128, 0.86f, 0.71f, 5.8f}, {kMx128x64, 128, 64, 0.60f, 0.44f, 5.f}, {kMx64x128, 64, 128, 0.60f, 0.44f, 5.f}, {kMx64x64, 64, 64, 0.57f, 0.31f, 5.f}};
 constexpr MxCost kMxRows4[] = {{kMx256x256, 256, 256, 0.99f, 0.99f, 9.5f}, {kMx256x192, 256, 192, 0.82f, 0.83f, 8.5f}, {kMx256x160, 256, 160, 0.72f, 0.74f, 8.f}, {kMx256x128, 256, 128, 0.58f, 0.53f, 7.f},
-                               {kMx128x128, 128, 128, 0.40f, 0.30f, 6.f}, {kMx128x64, 128, 64, 0.27f, 0.17f, 5.f}, {kMx64x64, 64, 64, 0.21f, 0.10f, 5.f}};
+                               {kMx128x128, 128, 128, 0.40f, 0.30f, 6.f}, {kMx128x64, 128, 64, 0.27f, 0.17f, 5.f}, {kMx64x128, 64, 128, 0.27f, 0.17f, 5.f}, {kMx64x64, 64, 64, 0.21f, 0.10f, 5.f}};
+constexpr int kMxStreamRows = 256;      // most rows that the streaming kernel is asked for
 
-// Which form a product of M rows with N rows of a matrix (gate and up together) takes: the matrix streamed for up to 64 rows, the tiles that the figures above foretell to be done first for more
-static int form_of(int64_t M, int64_t N, int k_tiles, int kind, bool gated, int shares) {
-  if (M <= 64) return kMxStream;
-  int best = kMx64x64;
-  float least = 0.f;
-  for (const MxCost& c : kind == kE2M1 ? kMxRows4 : kMxRows8) {
-    if (gated && c.form == kMx256x160) continue;
-    const int64_t blocks = mx_tiles(M, c.rows) * mx_tiles(N, c.columns) * shares, units = compute_units(), each = mx_tiles(blocks, units);
-    const float us = c.besides + 3.f * static_cast<float>(each - 1) + static_cast<float>(mx_tiles(k_tiles, shares)) * fmaxf(c.alone, static_cast<float>(each) * c.each);
-    if (least == 0.f || us < least) best = c.form, least = us;
+struct MxPlan {
+  int form, shares;
+  float us;
+};
+
+static int stream_tiles(int64_t M) { return M > 32 ? 4 : M > 16 ? 2 : 1; }
+
+// The quickest form for so many shares
+static MxPlan plan_for(int64_t M, int64_t N, int k_tiles, int kind, bool gated, int shares) {
+  MxPlan best = {kMx64x64, shares, 0.f};
+  const int64_t units = compute_units(), slabs = mx_tiles(k_tiles, shares);
+  if (M <= kMxStreamRows) {
+    const int mt = stream_tiles(M), waves = mt == 4 ? 4 : 8;
+    const int64_t blocks = mx_tiles(M, 16 * mt) * (gated ? mx_tiles(N, 64) : mx_tiles(N, 16 * mt)) * shares;
+    const float tile = gated ? (mt == 4 ? 1.9f : mt == 2 ? 1.8f : 1.4f) : mt == 4 ? 1.0f : mt == 2 ? 0.85f : 0.42f;
+    best = {kMxStream, shares, 4.5f + (kind == kE2M1 ? 0.6f : 1.f) * tile * static_cast<float>(mx_tiles(slabs, waves)) * static_cast<float>(mx_tiles(blocks, units))};
+  }
+  if (M > 16)
+    for (const MxCost& c : kind == kE2M1 ? kMxRows4 : kMxRows8) {
+      if (gated && c.form == kMx256x160) continue;
+      const int64_t blocks = mx_tiles(M, c.rows) * mx_tiles(N, c.columns) * shares, each = mx_tiles(blocks, units);
+      const float us = c.besides + 3.f * static_cast<float>(each - 1) + static_cast<float>(slabs) * fmaxf(c.alone, static_cast<float>(each) * c.each);
+      if (best.us == 0.f || us < best.us) best = {c.form, shares, us};
+    }
+  return best;
+}
+
+// ... and for any number of them
+static MxPlan plan_of(int64_t M, int64_t N, int k_tiles, int kind, bool norm_adds) {
+  MxPlan best = plan_for(M, N, k_tiles, kind, false, 1);
+  for (int shares : {2, 3, 4, 6, 8}) {
+    if (shares * 4 > k_tiles) break;
+    MxPlan p = plan_for(M, N, k_tiles, kind, false, shares);
+    p.us += static_cast<float>(shares) * static_cast<float>(M) * static_cast<float>(N) * 2e-6f + (norm_adds ? 0.5f : 3.5f);
+    if (p.us < best.us) best = p;
   }
   return best;
+}
+
+static int product_shares(void* out, int dtype, int64_t ldo, int shares, int64_t share_stride, const void* a, int a_kind, const void* w, const float* bias, int64_t M, int64_t N, int64_t K, int epilogue, int form,
+                          int vec, hipStream_t stream) {
+  const int k_tiles = static_cast<int>(mx_tiles(K, 128));
+  const MxMatrix ma = matrix_of(a, M, K, a_kind), mw = matrix_of(w, N, K, kE2M1);
+  if (form != kMxStream) return launch_mx_tiles(form, out, dtype, ldo, shares, share_stride, ma, a_kind, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec, stream);
+  // (as many tiles of the matrix as of rows: what is read of the rows, and e4m3 taken apart, serves them all)
+  const int mt = stream_tiles(M);
+  const dim3 grid((mw.tiles + mt - 1) / mt, (ma.tiles + mt - 1) / mt, shares);
+#define GO(T, ACT, MT, U) mx_stream_kernel<T, ACT, MT, MT, (MT == 4 ? 4 : 8), U><<<grid, (MT == 4 ? 256 : 512), 0, stream>>>(static_cast<T*>(out), ldo, share_stride, ma, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec)
+#define GO_MT(T, ACT) do { if (mt == 1) GO(T, ACT, 1, 3); else if (mt == 2) GO(T, ACT, 2, 2); else GO(T, ACT, 4, 1); } while (0)
+  if (dtype == kF32) { if (a_kind == kE2M1) GO_MT(float, kE2M1); else GO_MT(float, kE4M3); }
+  else { if (a_kind == kE2M1) GO_MT(bf16_t, kE2M1); else GO_MT(bf16_t, kE4M3); }
+#undef GO_MT
+#undef GO
+  return check_launch("gemm_mx");
 }
 
 }  // namespace alofa
 
 using namespace alofa;
 
-// out (dtype) = a w^T (+ bias), or += with the residual epilogue (float). shares > 1: `out` is [shares, M, N] floats, share_stride apart, each the sum over a part of K.
-extern "C" int alofa_gemm_mx(void* out, int dtype, int64_t ldo, int shares, int64_t share_stride, const void* a, int a_kind, const void* w, const float* bias, int64_t M, int64_t N, int64_t K,
+// Into how many shares of K the product of M rows of a kind with an [N, K] matrix is cut: by alofa_gemm_mx, whose `parts` then has room for [shares, M, N] floats; or where a norm adds them up
+extern "C" int alofa_gemm_mx_shares(int64_t M, int64_t N, int64_t K, int kind, int norm_adds) {
+  return M < 1 || N < 1 || K < 1 || K > (1 << 24) ? 1 : plan_of(M, N, static_cast<int>(mx_tiles(K, 128)), kind, norm_adds != 0).shares;
+}
+
+// out (dtype) = a w^T (+ bias), or += with the residual epilogue (float). shares > 1: the sums over as many parts of K are left in `parts` [shares, M, N]; with `out` they are added up from there.
+extern "C" int alofa_gemm_mx(void* out, int dtype, int64_t ldo, int shares, float* parts, const void* a, int a_kind, const void* w, const float* bias, int64_t M, int64_t N, int64_t K,
                              int epilogue, int form, hipStream_t stream) {
   if (!product_fits("gemm_mx", a, a_kind, w, M, N, K)) return 1;
-  ALOFA_REQUIRE(out && (dtype == kF32 || dtype == kBF16) && ldo >= 0 && (epilogue == kMxStore || (epilogue == kMxResidual && dtype == kF32 && !bias)), "gemm_mx: output does not fit: dtype=%d epilogue=%d", dtype, epilogue);
-  ALOFA_REQUIRE(shares >= 1 && shares <= mx_tiles(K, 128) && (shares == 1 || (dtype == kF32 && epilogue == kMxStore && !bias)), "gemm_mx: shares=%d K=%lld", shares, static_cast<long long>(K));
+  ALOFA_REQUIRE((out || parts) && (dtype == kF32 || dtype == kBF16) && ldo >= 0 && (epilogue == kMxStore || (epilogue == kMxResidual && dtype == kF32 && !bias)), "gemm_mx: output does not fit: dtype=%d epilogue=%d", dtype, epilogue);
   const int k_tiles = static_cast<int>(mx_tiles(K, 128));
-  const MxMatrix ma = matrix_of(a, M, K, a_kind), mw = matrix_of(w, N, K, kE2M1);
-  const int vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && ldo % (dtype == kF32 ? 4 : 8) == 0 && (shares == 1 || share_stride % 4 == 0);
+  ALOFA_REQUIRE(shares >= 1 && shares <= k_tiles && (out == nullptr || (shares > 1) == (parts != nullptr)) && reinterpret_cast<uintptr_t>(parts) % 16 == 0, "gemm_mx: shares=%d K=%lld", shares, static_cast<long long>(K));
   ALOFA_REQUIRE(form >= -1 && form < kMxForms, "gemm_mx: form=%d", form);
-  if (form < 0) form = form_of(M, N, k_tiles, a_kind, false, shares);
-  if (form != kMxStream) return launch_mx_tiles(form, out, dtype, ldo, shares, share_stride, ma, a_kind, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec, stream);
-  const int mt = ma.tiles >= 4 ? 4 : ma.tiles >= 2 ? 2 : 1;
-  const dim3 grid(mw.tiles, (ma.tiles + mt - 1) / mt, shares);
-#define GO(T, ACT, MT) mx_stream_kernel<T, ACT, MT, 8, 4><<<grid, 512, 0, stream>>>(static_cast<T*>(out), ldo, share_stride, ma, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec)
-#define GO_MT(T, ACT) do { if (mt == 1) GO(T, ACT, 1); else if (mt == 2) GO(T, ACT, 2); else GO(T, ACT, 4); } while (0)
-  if (dtype == kF32) { if (a_kind == kE2M1) GO_MT(float, kE2M1); else GO_MT(float, kE4M3); }
-  else { if (a_kind == kE2M1) GO_MT(bf16_t, kE2M1); else GO_MT(bf16_t, kE4M3); }
-#undef GO_MT
-#undef GO
-  return check_launch("gemm_mx");
+  if (form < 0) form = plan_for(M, N, k_tiles, a_kind, false, shares).form;
+  auto aligned = [](const void* p, int64_t ld, int code) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (code == kF32 ? 4 : 8) == 0; };
+  const int out_vec = out && aligned(out, ldo, dtype);
+  if (parts) {
+    const int rc = product_shares(parts, kF32, N, shares, M * N, a, a_kind, w, nullptr, M, N, K, kMxStore, form, N % 4 == 0, stream);
+    if (rc || !out) return rc;
+    const int64_t blocks = mx_tiles(M * mx_tiles(N, 4), 256);
+    ALOFA_REQUIRE(blocks < 1 << 24, "gemm_mx: more outputs than a launch takes: M=%lld N=%lld", static_cast<long long>(M), static_cast<long long>(N));
+    if (dtype == kF32) mx_sum_kernel<float><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<float*>(out), ldo, parts, shares, bias, static_cast<int>(M), static_cast<int>(N), epilogue, out_vec);
+    else mx_sum_kernel<bf16_t><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<bf16_t*>(out), ldo, parts, shares, bias, static_cast<int>(M), static_cast<int>(N), epilogue, out_vec);
+    return check_launch("gemm_mx");
+  }
+  return product_shares(out, dtype, ldo, 1, 0, a, a_kind, w, bias, M, N, K, epilogue, form, out_vec, stream);
 }
 
 // out (microscaled rows [M, N]) = act(a gate^T) * (a up^T)
@@ -228,12 +343,12 @@ extern "C" int alofa_gemm_swiglu_mx(void* out, int out_kind, const void* a, int 
   const MxMatrix ma = matrix_of(a, M, K, a_kind), mg = matrix_of(gate, N, K, kE2M1), mu = matrix_of(up, N, K, kE2M1);
   const int64_t at = mx_scales_at(M, N, out_kind);
   ALOFA_REQUIRE(form >= -1 && form < kMxForms, "gemm_swiglu_mx: form=%d", form);
-  if (form < 0) form = form_of(M, 256 * static_cast<int64_t>(out_tiles), k_tiles, a_kind, true, 1);
+  if (form < 0) form = plan_for(M, 256 * static_cast<int64_t>(out_tiles), k_tiles, a_kind, true, 1).form;
   if (form != kMxStream) return launch_mx_tiles_gated(form, static_cast<uint8_t*>(out), out_kind, at, out_tiles, ma, a_kind, mg, mu, static_cast<int>(M), static_cast<int>(N), k_tiles, gelu != 0, stream);
-  const int mt = ma.tiles >= 2 ? 2 : 1;
+  const int mt = stream_tiles(M);
   const dim3 grid(4 * out_tiles, (ma.tiles + mt - 1) / mt);
-#define GO(ACT, OUT, MT) mx_stream_gated_kernel<ACT, OUT, MT, 8, 2><<<grid, 512, 0, stream>>>(static_cast<uint8_t*>(out), at, out_tiles, ma, mg, mu, static_cast<int>(M), static_cast<int>(N), k_tiles, gelu)
-#define GO_MT(ACT, OUT) do { if (mt == 1) GO(ACT, OUT, 1); else GO(ACT, OUT, 2); } while (0)
+#define GO(ACT, OUT, MT) mx_stream_gated_kernel<ACT, OUT, MT, (MT == 4 ? 4 : 8), (MT == 1 ? 2 : 1)><<<grid, (MT == 4 ? 256 : 512), 0, stream>>>(static_cast<uint8_t*>(out), at, out_tiles, ma, mg, mu, static_cast<int>(M), static_cast<int>(N), k_tiles, gelu)
+#define GO_MT(ACT, OUT) do { if (mt == 1) GO(ACT, OUT, 1); else if (mt == 2) GO(ACT, OUT, 2); else GO(ACT, OUT, 4); } while (0)
   if (a_kind == kE2M1) { if (out_kind == kE2M1) GO_MT(kE2M1, kE2M1); else GO_MT(kE2M1, kE4M3); }
   else { if (out_kind == kE2M1) GO_MT(kE4M3, kE2M1); else GO_MT(kE4M3, kE4M3); }
 #undef GO_MT

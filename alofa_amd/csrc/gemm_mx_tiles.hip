@@ -199,14 +199,18 @@ __device__ __forceinline__ void mx_tile_rows(const f32x16* const (&acc)[G], char
   const int r0 = lane / kLanes, n = n0 + lane % kLanes * kEach;
   const char* from = room + r0 * kRow + lane % kLanes * 16;
   TO* to = out + static_cast<int64_t>(m0 + r0) * ldo + n;
-  if (vec && n0 + 32 * G <= N && m0 + 32 <= M) {      // (uniform: whole tiles)
+  if (n >= N) return;
+  const int last = M - m0 - r0;      // rows of this lane's steps of kAtOnce
+  if (vec && n + kEach <= N) {
     if constexpr (sizeof(TO) == 4) {
       if (epilogue == kMxResidual) {
         float4 old[kTimes];
 #pragma unroll
-        for (int t = 0; t < kTimes; ++t) old[t] = *reinterpret_cast<const float4*>(to + static_cast<int64_t>(t * kAtOnce) * ldo);
+        for (int t = 0; t < kTimes; ++t)
+          if (t * kAtOnce < last) old[t] = *reinterpret_cast<const float4*>(to + static_cast<int64_t>(t * kAtOnce) * ldo);
 #pragma unroll
         for (int t = 0; t < kTimes; ++t) {
+          if (t * kAtOnce >= last) break;
           const float4 v = *reinterpret_cast<const float4*>(from + t * kAtOnce * kRow);
           *reinterpret_cast<float4*>(to + static_cast<int64_t>(t * kAtOnce) * ldo) = make_float4(old[t].x + v.x, old[t].y + v.y, old[t].z + v.z, old[t].w + v.w);
         }
@@ -214,15 +218,14 @@ __device__ __forceinline__ void mx_tile_rows(const f32x16* const (&acc)[G], char
       }
     }
 #pragma unroll
-    for (int t = 0; t < kTimes; ++t) *reinterpret_cast<uint4*>(to + static_cast<int64_t>(t * kAtOnce) * ldo) = *reinterpret_cast<const uint4*>(from + t * kAtOnce * kRow);
+    for (int t = 0; t < kTimes; ++t)
+      if (t * kAtOnce < last) *reinterpret_cast<uint4*>(to + static_cast<int64_t>(t * kAtOnce) * ldo) = *reinterpret_cast<const uint4*>(from + t * kAtOnce * kRow);
     return;
   }
-  for (int t = 0; t < kTimes; ++t) {
-    if (m0 + r0 + t * kAtOnce >= M) return;
+  for (int t = 0; t * kAtOnce < last && t < kTimes; ++t) {
     const TO* v = reinterpret_cast<const TO*>(from + t * kAtOnce * kRow);
     TO* row = to + static_cast<int64_t>(t * kAtOnce) * ldo;
-    for (int e = 0; e < kEach; ++e) {
-      if (n + e >= N) break;
+    for (int e = 0; e < kEach && n + e < N; ++e) {
       if (sizeof(TO) == 4 && epilogue == kMxResidual) store_f32(row + e, load_f32(row + e) + load_f32(v + e));
       else row[e] = v[e];
     }
@@ -332,6 +335,7 @@ template <int kAct> using T256x160 = MxTile<kAct, 5, 1, 1, 8, 3>;
 template <int kAct> using T256x128 = MxTile<kAct, 4, 1, 1, 8, 3>;
 template <int kAct> using T128x128 = MxTile<kAct, 4, 1, 1, 4, 3>;
 template <int kAct> using T128x64 = MxTile<kAct, 2, 1, 1, 4, 3>;
+template <int kAct> using T64x128 = MxTile<kAct, 2, 1, 2, 2, 4>;
 template <int kAct> using T64x64 = MxTile<kAct, 2, 1, 1, 2, 4>;
 
 }  // namespace
@@ -346,6 +350,7 @@ static int by_form(int form, void* out, int64_t ldo, int shares, int64_t share_s
     case kMx256x128: GO(T256x128);
     case kMx128x128: GO(T128x128);
     case kMx128x64: GO(T128x64);
+    case kMx64x128: GO(T64x128);
     default: GO(T64x64);
   }
 #undef GO
@@ -368,6 +373,7 @@ static int by_form_gated(int form, uint8_t* out, int64_t at, int out_tiles, cons
     case kMx256x128: GO(T256x128);
     case kMx128x128: GO(T128x128);
     case kMx128x64: GO(T128x64);
+    case kMx64x128: GO(T64x128);
     case kMx64x64: GO(T64x64);
     default: set_error("gemm_swiglu_mx: gate and up do not share tiles of this form: %d", form); return 1;
   }

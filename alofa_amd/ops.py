@@ -2960,7 +2960,7 @@ def rmsnorm_mx(out: MXRows, x: torch.Tensor, w: torch.Tensor, eps: float, add: O
     _call("alofa_rmsnorm_mx", out.buffer, kind, x, ldx, add, shares, stride, ld_add, total, ld_total, w, _F(eps), out.rows, out.k, _stream())
 
 
-MX_FORMS = {None: -1, "stream": 0, "256x256": 1, "256x192": 2, "256x160": 3, "256x128": 4, "128x128": 5, "128x64": 6, "64x64": 7}      # (as csrc/gemm_mx.h numbers them: the streaming kernel, or tiles of rows x columns)
+MX_FORMS = {None: -1, "stream": 0, "256x256": 1, "256x192": 2, "256x160": 3, "256x128": 4, "128x128": 5, "128x64": 6, "64x64": 7, "64x128": 8}      # (as csrc/gemm_mx.h numbers them: the streaming kernel, or tiles of rows x columns)
 
 
 def _mx_form(kernel: Optional[str]) -> int:
@@ -2979,13 +2979,20 @@ def _mx_product(a, w, matrices: str = "w") -> tuple:
     return kind, a.rows, w.rows, a.k
 
 
-def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor] = None, add_to_out: bool = False, kernel: Optional[str] = None) -> None:
+def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor] = None, add_to_out: bool = False, kernel: Optional[str] = None, scratch=None) -> None:
     """out [M, N] = a @ w.T (+ bias), float32 or bfloat16, or out += a @ w.T when ``add_to_out`` (out is then the float32 residual stream). ``a``: microscaled rows of either kind;
-    ``w``: a matrix [N, K] of e2m1. Sums in float32. ``kernel`` names one of ``MX_FORMS`` instead of the rule by sizes (csrc/gemm_mx.hip)."""
+    ``w``: a matrix [N, K] of e2m1. Sums in float32. ``kernel`` names one of ``MX_FORMS`` instead of the rule by sizes (csrc/gemm_mx.hip). ``scratch``: as for ``gemm``; without it, a product whose
+    sum is shared out over K allocates the shares."""
     kind, M, N, K = _mx_product(a, w)
-    form = -1 if kernel is None else _mx_form(kernel)
+    form, shares, parts = -1, 1, None
+    if kernel is not None:
+        form = _mx_form(kernel)
+    elif M > 16 or K > 8192:
+        shares = _answer("alofa_gemm_mx_shares", M, N, K, kind, 0)
     if _here() == a.device == w.device and (sizes := _native().mx_matrix(out, bias, M, N, a.device, 1)) is not None and (not add_to_out or (bias is None and sizes[0] == F32)):
-        _call("alofa_gemm_mx", out, *sizes, 1, 0, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, form, _stream())
+        if shares > 1:
+            parts = torch.empty(shares * M * N, dtype=torch.float32, device=out.device) if scratch is None else scratch("mx_sums", (shares * M * N,), torch.float32)
+        _call("alofa_gemm_mx", out, *sizes, shares, parts, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, form, _stream())
         return
     _gpu("out", out, None, 2)
     if tuple(out.shape) != (M, N):
@@ -3000,12 +3007,14 @@ def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor
         raise AlofaError("unsupported", "a product that adds to the residual stream takes no bias; add the bias in a buffer of its own")
     code, ldo = dtype_code(out), _out_rows("out", out)
     _one_device(out, a.buffer, w.buffer, bias)
-    _call("alofa_gemm_mx", out, code, ldo, 1, 0, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, form, _stream())
+    if shares > 1:
+        parts = torch.empty(shares * M * N, dtype=torch.float32, device=out.device) if scratch is None else scratch("mx_sums", (shares * M * N,), torch.float32)
+    _call("alofa_gemm_mx", out, code, ldo, shares, parts, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, form, _stream())
 
 
-def mx_shares(M: int, N: int, K: int) -> int:
-    """Into how many shares of K the product of so many rows with an [N, K] matrix is best cut where ``rmsnorm_mx`` adds them up."""
-    return 1
+def mx_shares(M: int, N: int, K: int, kind: str = "e4m3") -> int:
+    """Into how many shares of K the product of so many rows of ``kind`` with an [N, K] matrix is best cut where ``rmsnorm_mx`` adds them up."""
+    return _answer("alofa_gemm_mx_shares", M, N, K, MX_KINDS[kind], 1)
 
 
 def gemm_mx_shares(out: torch.Tensor, a: MXRows, w: MXRows, kernel: Optional[str] = None) -> None:
@@ -3015,7 +3024,9 @@ def gemm_mx_shares(out: torch.Tensor, a: MXRows, w: MXRows, kernel: Optional[str
     if tuple(out.shape[1:]) != (M, N) or not 1 <= out.shape[0] <= (K + 127) // 128:
         raise AlofaError("shape_mismatch", "the shares of a product do not fit", f"a={a} w={w} out={tuple(out.shape)}")
     _one_device(out, a.buffer, w.buffer)
-    _call("alofa_gemm_mx", out, F32, N, out.shape[0], M * N, a.buffer, kind, w.buffer, None, M, N, K, STORE, _mx_form(kernel), _stream())
+    if out.data_ptr() % 16:
+        raise AlofaError("shape_mismatch", "the shares of a product begin at a 16-byte place", f"address={out.data_ptr():#x}")
+    _call("alofa_gemm_mx", None, F32, N, out.shape[0], out, a.buffer, kind, w.buffer, None, M, N, K, STORE, _mx_form(kernel), _stream())
 
 
 def gemm_swiglu_mx(out: MXRows, a: MXRows, w_gate: MXRows, w_up: MXRows, act: str = "silu", kernel: Optional[str] = None) -> None:

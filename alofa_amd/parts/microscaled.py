@@ -60,21 +60,21 @@ class MicroscaledPreNorm(PreNormBlock):
         normed = self._rows(ctx, "mx_normed", T, h)
         ops.rmsnorm_mx(normed, hidden, *self.norms[0].as_rmsnorm())
         qkv = ctx.scratch("qkv", (T, m.qkv_width), self.rt.dtype)
-        ops.gemm_mx(qkv, normed, self.w_qkv, m.b_qkv)
+        ops.gemm_mx(qkv, normed, self.w_qkv, m.b_qkv, scratch=ctx.scratch)
         attn = ctx.scratch("attn", (T, m.heads * m.d), self.rt.dtype)
         paged_attend(ctx, entry, qkv, attn, m.heads, m.kv_heads, m.d, m.window, m.scale, m.position, self.rt)
         rows = self._rows(ctx, "mx_attn", T, m.heads * m.d)
         ops.mx_quantize(rows, attn)
         if m.b_o is not None:
             mixed = ctx.scratch("attn_proj", (T, h), torch.float32)
-            ops.gemm_mx(mixed, rows, self.w_o, m.b_o)
+            ops.gemm_mx(mixed, rows, self.w_o, m.b_o, scratch=ctx.scratch)
         else:
             mixed = ctx.scratch("mx_shares", (ops.mx_shares(T, h, rows.k), T, h), torch.float32)
             ops.gemm_mx_shares(mixed, rows, self.w_o)
         ops.rmsnorm_mx(normed, hidden, *self.norms[1].as_rmsnorm(), add=mixed, total=hidden)
         act = self._rows(ctx, "mx_act", T, f.intermediate)
         ops.gemm_swiglu_mx(act, normed, self.w_gate, self.w_up, f.activation)
-        ops.gemm_mx(hidden, act, self.w_down, add_to_out=True)
+        ops.gemm_mx(hidden, act, self.w_down, add_to_out=True, scratch=ctx.scratch)
 
 
 register_part("block", KIND, MicroscaledPreNorm)
