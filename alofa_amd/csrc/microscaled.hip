@@ -36,49 +36,82 @@ __device__ __forceinline__ void put8(uint8_t* __restrict__ out, int64_t scales_a
   if (c % 4 == 0) out[scales_at + mx_scale_place(r, c / 4, k_tiles)] = static_cast<uint8_t>(code);
 }
 
-// ---- numbers to microscaled rows ---------------------------------------------
-// A thread takes eight numbers of one row; four neighbours make a block.
+// ---- numbers to microscaled rows and back --------------------------------------
+// A block takes 16 rows by 512 columns, four tiles: a wave has four of the rows, a lane eight numbers of each. The tiles are put together in LDS and leave as whole runs (row by row, 16 bytes of each 256 would be
+// written at a time).
+constexpr int kStrip = 4;      // tiles along a row that a block takes
+
 template <typename T, int kKind, bool kVec>
-__global__ void __launch_bounds__(256) mx_quantize_kernel(uint8_t* __restrict__ out, int64_t scales_at, const T* __restrict__ x, int64_t ldx, int rows, int k, int k_tiles) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int per_row = 16 * k_tiles;
-  const int64_t r = i / per_row;
-  const int c = static_cast<int>(i % per_row);
-  if (r >= rows) return;      // (a row's threads are a multiple of four)
-  float v[8];
-  load8<T, kVec>(x + r * ldx, 8 * c, k, v);
-  put8<kKind>(out, scales_at, r, c, k_tiles, v);
+__global__ void __launch_bounds__(256) mx_quantize_kernel(uint8_t* __restrict__ out, int64_t scales_at, const T* __restrict__ x, int64_t ldx, int rows, int k, int k_tiles, int strips) {
+  constexpr int kTile = mx_units(kKind) * 16;
+  __shared__ __attribute__((aligned(16))) uint8_t tiles[kStrip * kTile];
+  __shared__ __attribute__((aligned(16))) uint8_t scales[kStrip * 64];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, row_tile = blockIdx.x / strips, strip = blockIdx.x % strips, c = strip * kStrip * 16 + lane;
+  float v[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = static_cast<int64_t>(row_tile) * 16 + 4 * wave + i;
+    if (r < rows) load8<T, kVec>(x + r * ldx, 8 * c, k, v[i]);
+    else
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) put8<kKind>(tiles, scales - tiles, 4 * wave + i, lane, kStrip, v[i]);
+  __syncthreads();
+  const int64_t first = static_cast<int64_t>(row_tile) * k_tiles + strip * kStrip;
+  const int there = min(kStrip, k_tiles - strip * kStrip);
+  for (int i = threadIdx.x; i < there * (kTile / 16); i += 256) reinterpret_cast<uint4*>(out + first * kTile)[i] = reinterpret_cast<const uint4*>(tiles)[i];
+  if (static_cast<int>(threadIdx.x) < there * 4) reinterpret_cast<uint4*>(out + scales_at + first * 64)[threadIdx.x] = reinterpret_cast<const uint4*>(scales)[threadIdx.x];
 }
 
-// ---- the values that microscaled rows stand for --------------------------------
 __device__ __forceinline__ float mx_scaled(float element, uint32_t code) { return code == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(element, static_cast<int>(code) - 127); }
 
-template <typename T, int kKind>
-__global__ void __launch_bounds__(256) mx_values_kernel(T* __restrict__ out, int64_t ldo, const uint8_t* __restrict__ q, int64_t scales_at, int rows, int k, int k_tiles) {
+template <typename T, int kKind, bool kVec>
+__global__ void __launch_bounds__(256) mx_values_kernel(T* __restrict__ out, int64_t ldo, const uint8_t* __restrict__ q, int64_t scales_at, int rows, int k, int k_tiles, int strips) {
   typedef float f32x2_t __attribute__((ext_vector_type(2)));
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int per_row = 16 * k_tiles;
-  const int64_t r = i / per_row;
-  const int c = static_cast<int>(i % per_row);
-  if (r >= rows || 8 * c >= k) return;
-  const uint32_t code = q[scales_at + mx_scale_place(r, c / 4, k_tiles)];
-  const uint8_t* at = q + mx_place8<kKind>(r, c, k_tiles);
-  float v[8];
-  if constexpr (kKind == kE2M1) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(at);
-    const f32x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1);
-    const f32x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
-    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = d[0], v[5] = d[1], v[6] = e[0], v[7] = e[1];
-  } else {
-    const uint2 w = *reinterpret_cast<const uint2*>(at);
-    const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, true);
-    const f32x2_t d = __builtin_amdgcn_cvt_pk_f32_fp8(w.y, false), e = __builtin_amdgcn_cvt_pk_f32_fp8(w.y, true);
-    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = d[0], v[5] = d[1], v[6] = e[0], v[7] = e[1];
-  }
-  T* to = out + r * ldo + 8 * c;
+  constexpr int kTile = mx_units(kKind) * 16;
+  __shared__ __attribute__((aligned(16))) uint8_t tiles[kStrip * kTile];
+  __shared__ __attribute__((aligned(16))) uint8_t scales[kStrip * 64];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, row_tile = blockIdx.x / strips, strip = blockIdx.x % strips, c = strip * kStrip * 16 + lane;
+  const int64_t first = static_cast<int64_t>(row_tile) * k_tiles + strip * kStrip;
+  const int there = min(kStrip, k_tiles - strip * kStrip);
+  for (int i = threadIdx.x; i < there * (kTile / 16); i += 256) reinterpret_cast<uint4*>(tiles)[i] = reinterpret_cast<const uint4*>(q + first * kTile)[i];
+  if (static_cast<int>(threadIdx.x) < there * 4) reinterpret_cast<uint4*>(scales)[threadIdx.x] = reinterpret_cast<const uint4*>(q + scales_at + first * 64)[threadIdx.x];
+  __syncthreads();
+  if (8 * c >= k) return;
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (8 * c + e < k) store_f32(to + e, mx_scaled(v[e], code));
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = static_cast<int64_t>(row_tile) * 16 + 4 * wave + i;
+    if (r >= rows) return;
+    const uint32_t code = scales[mx_scale_place(4 * wave + i, lane / 4, kStrip)];
+    const uint8_t* at = tiles + mx_place8<kKind>(4 * wave + i, lane, kStrip);
+    float v[8];
+    if constexpr (kKind == kE2M1) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(at);
+      const f32x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1);
+      const f32x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
+      v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = d[0], v[5] = d[1], v[6] = e[0], v[7] = e[1];
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2*>(at);
+      const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w.x, true);
+      const f32x2_t d = __builtin_amdgcn_cvt_pk_f32_fp8(w.y, false), e = __builtin_amdgcn_cvt_pk_f32_fp8(w.y, true);
+      v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = d[0], v[5] = d[1], v[6] = e[0], v[7] = e[1];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = mx_scaled(v[e], code);
+    T* to = out + r * ldo + 8 * c;
+    if constexpr (kVec && sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    } else if constexpr (kVec) {
+      *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (8 * c + e < k) store_f32(to + e, v[e]);
+    }
+  }
 }
 
 // ---- a checkpoint's codes, row by row, into the order above --------------------
@@ -116,6 +149,22 @@ __device__ __forceinline__ float round_to_odd(double y) {
   return y != y ? f : __uint_as_float(u);
 }
 
+// sum += add[1] + add[2] + .. in this order, three shares' loads on their way together
+template <bool kVec>
+__device__ __forceinline__ void add_shares(const float* __restrict__ row, int64_t share_stride, int shares, int c0, int k, float (&sum)[8]) {
+  for (int s = 1; s < shares; s += 3) {
+    float part[3][8];
+#pragma unroll
+    for (int u = 0; u < 3; ++u) load8<float, kVec>(row + min(s + u, shares - 1) * share_stride, c0, k, part[u]);
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+      if (s + u < shares) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += part[u][e];
+      }
+  }
+}
+
 // total = x + (add[0] + add[1] + ..) in float, y = total / sqrt(mean(total^2) + eps) * w in double, y to microscaled rows. A block takes a row. The squares' sum and
 // y are in double so that no element depends on the order of a sum: a value next to the middle of two elements would become one or the other.
 // kGroups > 0: a row of at most 2,048 kGroups numbers stays in registers between the sum and the scaling; 0: any row, read twice.
@@ -130,12 +179,7 @@ __global__ void __launch_bounds__(256) rmsnorm_mx_kernel(uint8_t* __restrict__ o
     if (shares == 0) return;
     float sum[8];
     load8<float, kVec>(add + r * ld_add, 8 * c, k, sum);
-    for (int s = 1; s < shares; ++s) {
-      float part[8];
-      load8<float, kVec>(add + s * share_stride + r * ld_add, 8 * c, k, part);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += part[e];
-    }
+    add_shares<kVec>(add + r * ld_add, share_stride, shares, 8 * c, k, sum);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += sum[e];
   };
@@ -151,16 +195,16 @@ __global__ void __launch_bounds__(256) rmsnorm_mx_kernel(uint8_t* __restrict__ o
         if (8 * c + e < k) to[e] = v[e];
     }
   };
-  auto leave = [&](int c, float (&v)[8], double scale) {
-    float weight[8];
-    load8<float, kVec>(w, 8 * c, k, weight);
+  auto leave = [&](int c, float (&v)[8], const float (&weight)[8], double scale) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = round_to_odd(static_cast<double>(v[e]) * scale * static_cast<double>(weight[e]));
     put8<kKind>(out, scales_at, r, c, k_tiles, v);
   };
   double ss = 0;
   if constexpr (kGroups > 0) {
-    float v[kGroups][8];
+    float v[kGroups][8], weight[kGroups][8];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) load8<float, kVec>(w, 8 * (static_cast<int>(threadIdx.x) + 256 * i), k, weight[i]);
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
       const int c = threadIdx.x + 256 * i;
@@ -174,7 +218,7 @@ __global__ void __launch_bounds__(256) rmsnorm_mx_kernel(uint8_t* __restrict__ o
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
       const int c = threadIdx.x + 256 * i;
-      if (c < per_row) leave(c, v[i], scale);
+      if (c < per_row) leave(c, v[i], weight[i], scale);
     }
   } else {
     for (int c = threadIdx.x; c < per_row; c += 256) {
@@ -189,7 +233,9 @@ __global__ void __launch_bounds__(256) rmsnorm_mx_kernel(uint8_t* __restrict__ o
       float v[8];
       take(c, v);      // (`total` may be x itself: a thread reads its numbers again before it writes them)
       keep(c, v);
-      leave(c, v, scale);
+      float weight[8];
+      load8<float, kVec>(w, 8 * c, k, weight);
+      leave(c, v, weight, scale);
     }
   }
 }
@@ -213,10 +259,11 @@ extern "C" int alofa_mx_quantize(void* out, int kind, const void* x, int dtype, 
   ALOFA_REQUIRE(out && x && aligned16(out) && (dtype == kF32 || dtype == kBF16) && ldx >= 0, "mx_quantize: operands do not fit: dtype=%d ldx=%lld", dtype, static_cast<long long>(ldx));
   const int k_tiles = static_cast<int>(mx_tiles(k, 128));
   const int64_t at = mx_scales_at(rows, k, kind);
-  const unsigned blocks = static_cast<unsigned>(mx_tiles(rows * 16 * k_tiles, 256));
+  const int strips = (k_tiles + kStrip - 1) / kStrip;
+  const unsigned blocks = static_cast<unsigned>(mx_tiles(rows, 16) * strips);
   const bool vec = aligned16(x) && k % 8 == 0 && ldx % (dtype == kF32 ? 4 : 8) == 0;
   const int r = static_cast<int>(rows), n = static_cast<int>(k);
-#define GO(T, KIND, VEC) mx_quantize_kernel<T, KIND, VEC><<<blocks, 256, 0, stream>>>(static_cast<uint8_t*>(out), at, static_cast<const T*>(x), ldx, r, n, k_tiles)
+#define GO(T, KIND, VEC) mx_quantize_kernel<T, KIND, VEC><<<blocks, 256, 0, stream>>>(static_cast<uint8_t*>(out), at, static_cast<const T*>(x), ldx, r, n, k_tiles, strips)
 #define GO_VEC(T, KIND) do { if (vec) GO(T, KIND, true); else GO(T, KIND, false); } while (0)
   if (dtype == kF32) { if (kind == kE2M1) GO_VEC(float, kE2M1); else GO_VEC(float, kE4M3); }
   else { if (kind == kE2M1) GO_VEC(bf16_t, kE2M1); else GO_VEC(bf16_t, kE4M3); }
@@ -228,13 +275,16 @@ extern "C" int alofa_mx_quantize(void* out, int kind, const void* x, int dtype, 
 extern "C" int alofa_mx_values(void* out, int dtype, int64_t ldo, const void* q, int kind, int64_t rows, int64_t k, hipStream_t stream) {
   if (!sizes_fit("mx_values", kind, rows, k)) return 1;
   ALOFA_REQUIRE(out && q && aligned16(q) && (dtype == kF32 || dtype == kBF16) && ldo >= 0, "mx_values: operands do not fit: dtype=%d ldo=%lld", dtype, static_cast<long long>(ldo));
-  const int k_tiles = static_cast<int>(mx_tiles(k, 128));
+  const int k_tiles = static_cast<int>(mx_tiles(k, 128)), strips = (k_tiles + kStrip - 1) / kStrip;
   const int64_t at = mx_scales_at(rows, k, kind);
-  const unsigned blocks = static_cast<unsigned>(mx_tiles(rows * 16 * k_tiles, 256));
+  const unsigned blocks = static_cast<unsigned>(mx_tiles(rows, 16) * strips);
+  const bool vec = aligned16(out) && k % 8 == 0 && ldo % (dtype == kF32 ? 4 : 8) == 0;
   const int r = static_cast<int>(rows), n = static_cast<int>(k);
-#define GO(T, KIND) mx_values_kernel<T, KIND><<<blocks, 256, 0, stream>>>(static_cast<T*>(out), ldo, static_cast<const uint8_t*>(q), at, r, n, k_tiles)
-  if (dtype == kF32) { if (kind == kE2M1) GO(float, kE2M1); else GO(float, kE4M3); }
-  else { if (kind == kE2M1) GO(bf16_t, kE2M1); else GO(bf16_t, kE4M3); }
+#define GO(T, KIND, VEC) mx_values_kernel<T, KIND, VEC><<<blocks, 256, 0, stream>>>(static_cast<T*>(out), ldo, static_cast<const uint8_t*>(q), at, r, n, k_tiles, strips)
+#define GO_VEC(T, KIND) do { if (vec) GO(T, KIND, true); else GO(T, KIND, false); } while (0)
+  if (dtype == kF32) { if (kind == kE2M1) GO_VEC(float, kE2M1); else GO_VEC(float, kE4M3); }
+  else { if (kind == kE2M1) GO_VEC(bf16_t, kE2M1); else GO_VEC(bf16_t, kE4M3); }
+#undef GO_VEC
 #undef GO
   return check_launch("mx_values");
 }
@@ -263,7 +313,7 @@ extern "C" int alofa_rmsnorm_mx(void* out, int kind, const float* x, int64_t ldx
   const int groups = (16 * k_tiles + 255) / 256;
 #define GO(KIND, G, VEC) rmsnorm_mx_kernel<KIND, G, VEC><<<static_cast<unsigned>(rows), 256, 0, stream>>>(static_cast<uint8_t*>(out), at, x, ldx, add, shares, share_stride, ld_add, total, ld_total, w, eps, n, k_tiles)
 #define GO_VEC(KIND, G) do { if (vec) GO(KIND, G, true); else GO(KIND, G, false); } while (0)
-#define GO_GROUPS(KIND) do { if (groups == 1) GO_VEC(KIND, 1); else if (groups == 2) GO_VEC(KIND, 2); else if (groups <= 4) GO_VEC(KIND, 4); else GO_VEC(KIND, 0); } while (0)
+#define GO_GROUPS(KIND) do { if (groups == 1) GO_VEC(KIND, 1); else if (groups == 2) GO_VEC(KIND, 2); else if (groups == 3) GO_VEC(KIND, 3); else if (groups == 4) GO_VEC(KIND, 4); else GO_VEC(KIND, 0); } while (0)
   if (kind == kE2M1) GO_GROUPS(kE2M1); else GO_GROUPS(kE4M3);
 #undef GO_GROUPS
 #undef GO_VEC
