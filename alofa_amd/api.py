@@ -34,7 +34,7 @@ class Engine:
                  memory_fraction: Optional[float] = None, matrices: str = "stored"):
         """``model``: a (config, Model) pair already on the device, instead of a folder to load.
         ``matrices``: "stored", or "mxfp4": the layers' matrices are held in 4 bits, a quarter of the memory that bfloat16 takes and that a decode step
-        reads (``load_model``; a ``model`` that is given is as it is).
+        reads (``load_model``; not with a ``model`` that is given).
         ``report``: a callable that receives one line about device memory at start (default:
         standard error when ALOFA_REPORT_MEMORY is set). ``run_ahead``: a tick reads the tokens of the
         tick before only after its own step is launched (``EngineCore``); off, every tick is synchronous.
@@ -46,6 +46,8 @@ class Engine:
         so that a lone long prompt takes one step (requests are served in order of arrival either way, and the
         budget alone bounds a tick's length)."""
         max_chunk = token_budget if max_chunk is None else max_chunk
+        if model is not None and matrices != "stored":
+            raise AlofaError("invalid_argument", "a model that is given holds its matrices as it does", f"matrices={matrices}")
         from .csrc.build import load
         load()
         self.config, self.model = model if model is not None else load_model(Path(model_dir), dtype, device, matrices)

@@ -206,9 +206,11 @@ static MxMatrix matrix_of(const void* p, int64_t rows, int64_t k, int kind) {
   return {at, at + mx_scales_at(rows, k, kind), static_cast<int>(mx_tiles(rows, 16))};
 }
 
+constexpr int64_t kMxMostRows = 65535 * 64;      // (what the streaming kernel's grid has room for)
+
 static bool product_fits(const char* what, const void* a, int a_kind, const void* w, int64_t M, int64_t N, int64_t K) {
   const bool ok = a && w && reinterpret_cast<uintptr_t>(a) % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 && (a_kind == kE2M1 || a_kind == kE4M3) && M >= 1 && N >= 1 && K >= 1 &&
-                  M <= (1 << 20) && N <= (1 << 24) && K <= (1 << 24);
+                  M <= kMxMostRows && N <= (1 << 24) && K <= (1 << 24);
   if (!ok) set_error("%s: operands do not fit: M=%lld N=%lld K=%lld kind=%d", what, static_cast<long long>(M), static_cast<long long>(N), static_cast<long long>(K), a_kind);
   return ok;
 }

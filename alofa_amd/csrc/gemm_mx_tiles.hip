@@ -315,14 +315,18 @@ namespace {
 template <typename TO, int kAct, typename T>
 int go(void* out, int64_t ldo, int shares, int64_t share_stride, const MxMatrix& a, const MxMatrix& w, const float* bias, int M, int N, int k_tiles, int epilogue, bool vec, hipStream_t stream) {
   const int tiles_m = (M + T::BM - 1) / T::BM, tiles_n = (N + T::BN - 1) / T::BN;
-  mx_tile_kernel<TO, kAct, T><<<static_cast<unsigned>(tiles_m) * tiles_n * shares, T::kWaves * 64, 0, stream>>>(static_cast<TO*>(out), ldo, share_stride, a, w, bias, M, N, k_tiles, tiles_m, tiles_n, shares, epilogue, vec);
+  const int64_t blocks = static_cast<int64_t>(tiles_m) * tiles_n * shares;
+  ALOFA_REQUIRE(blocks * T::kWaves * 64 < INT64_C(1) << 32, "gemm_mx: more tiles than a launch takes: M=%d N=%d shares=%d", M, N, shares);
+  mx_tile_kernel<TO, kAct, T><<<static_cast<unsigned>(blocks), T::kWaves * 64, 0, stream>>>(static_cast<TO*>(out), ldo, share_stride, a, w, bias, M, N, k_tiles, tiles_m, tiles_n, shares, epilogue, vec);
   return check_launch("gemm_mx");
 }
 
 template <int kAct, int kOut, typename T>
 int go_gated(uint8_t* out, int64_t at, int out_tiles, const MxMatrix& a, const MxMatrix& gate, const MxMatrix& up, int M, int N, int k_tiles, bool gelu, hipStream_t stream) {
   const int tiles_m = (M + T::BM - 1) / T::BM, tiles_n = (out_tiles * 128 + T::BN / 2 - 1) / (T::BN / 2);
-  const unsigned blocks = static_cast<unsigned>(tiles_m) * tiles_n;
+  const int64_t all = static_cast<int64_t>(tiles_m) * tiles_n;
+  ALOFA_REQUIRE(all * T::kWaves * 64 < INT64_C(1) << 32, "gemm_swiglu_mx: more tiles than a launch takes: M=%d N=%d", M, N);
+  const unsigned blocks = static_cast<unsigned>(all);
   if (gelu) mx_tile_gated_kernel<kAct, kOut, T, true><<<blocks, T::kWaves * 64, 0, stream>>>(out, at, out_tiles, a, gate, up, M, N, k_tiles, tiles_m, tiles_n);
   else mx_tile_gated_kernel<kAct, kOut, T, false><<<blocks, T::kWaves * 64, 0, stream>>>(out, at, out_tiles, a, gate, up, M, N, k_tiles, tiles_m, tiles_n);
   return check_launch("gemm_swiglu_mx");

@@ -92,3 +92,9 @@ def test_the_command_refuses_them_too(tiny_dirs, monkeypatch, dtype, matrices):
     with pytest.raises(AlofaError) as e:
         cli.main(["5,6"])
     assert "ALOFA_MATRICES" in str(e.value)
+
+
+def test_an_engine_over_a_given_model_does_not_change_its_matrices():
+    from alofa_amd import Engine
+    with pytest.raises(AlofaError):
+        Engine(None, model=(None, None), matrices="mxfp4")

@@ -152,6 +152,19 @@ def test_norm_rows_that_are_zero_or_not_finite_keep_to_themselves():
     assert np.isnan(got[2, :32]).all() and (got[2, 32:] == 0).all() and np.isnan(got[3]).all()
 
 
+def test_norm_of_very_large_and_very_small_rows():
+    x, w = numbers(6, 896, 3, 2), numbers(1, 896, 4, 0)[0]
+    x[1:3] *= np.float32(1e37)      # (squares beyond a float)
+    x[3:5] *= np.float32(1e-37)
+    w[:10] *= np.float32(1e30)
+    want = pm.rounded(pm.norm(x.astype(np.float64), w.astype(np.float64), 1e-6), "e4m3")
+    q = ops.MXRows(6, 896, "e4m3", DEV)
+    ops.rmsnorm_mx(q, on(x), on(w), 1e-6)
+    # (a scale is 2^-127 at least and an element 2^-9: what is below half of that is zero on both sides; below 2^-149 a float has no bits left)
+    got = read(q)
+    same(got, want.astype(np.float32).astype(np.float64))
+
+
 @pytest.mark.parametrize("k", [896, 5120])
 def test_norm_of_a_row_does_not_depend_on_the_others(k):
     x, w = numbers(300, k, 9, 2), numbers(1, k, 10, 0)[0]
@@ -223,6 +236,75 @@ def check_gated(out, av, gv, uv, act, out_kind):
     ops.gemm_mx(sums, out, ones)
     one = np.ones((1, N))
     assert (np.abs(sums.double().cpu().numpy() - got @ one.T) <= off_by(got, one)).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("M,N,K", [(5, 40, 256), (300, 200, 384)])
+def test_products_of_blocks_with_scales_far_apart(M, N, K, kind):
+    rng = np.random.default_rng(K)
+    blocks = K // 32
+    ea, ew = rng.integers(0, 251, (M, blocks)), rng.integers(-20, 21, (N, blocks))
+    ca = rng.integers(0, 16 if kind == "e2m1" else 256, (M, K))
+    if kind == "e4m3":
+        ca = np.where((ca & 127) == 127, 0, ca)      # (no NaN)
+    cw = rng.integers(0, 16, (N, K))
+    # rows' scales from end to end of the range, the matrix's so that every block's products come out around 2^0
+    ea = np.broadcast_to(rng.integers(2, 249, (1, blocks)), (M, blocks)) + rng.integers(-2, 3, (M, blocks))
+    ew = np.clip(254 - ea[:1] + ew, 0, 254)
+    pairs = lambda c: c[:, 0::2] | c[:, 1::2] << 4      # noqa: E731
+    to = lambda c: torch.from_numpy(np.ascontiguousarray(c.astype(np.uint8))).to(DEV)      # noqa: E731
+    a = ops.mx_from_codes(to(pairs(ca) if kind == "e2m1" else ca), to(ea), K, kind)
+    w = ops.mx_from_codes(to(pairs(cw)), to(ew), K)
+    av, wv = pm.values(ca, ea, K, kind), pm.values(cw, ew, K, "e2m1")
+    out = torch.empty(M, N, device=DEV)
+    ops.gemm_mx(out, a, w)
+    assert (np.abs(out.double().cpu().numpy() - av @ wv.T) <= off_by(av, wv)).all()
+
+
+def test_matrices_beyond_32_bits_of_bytes():
+    """The last rows of 2.4 GB of matrix, and of rows as long, against the same tiles as matrices of their own."""
+    N, K = 1_100_007, 4096
+    g = torch.Generator(DEV).manual_seed(1)
+
+    def tail(q, tiles):      # the last row tiles of q as rows of their own
+        per = -(-K // 128) * (1024 if q.kind == "e2m1" else 2048)
+        rows = q.rows - (-(-q.rows // 16) - tiles) * 16
+        t = ops.MXRows(rows, K, q.kind, DEV)
+        all_tiles, scales = -(-q.rows // 16), -(-K // 128) * 64
+        t.buffer[:tiles * per] = q.buffer[(all_tiles - tiles) * per:all_tiles * per]
+        t.buffer[tiles * per:tiles * (per + scales)] = q.buffer[all_tiles * per + (all_tiles - tiles) * scales:all_tiles * (per + scales)]
+        return t
+
+    w = ops.MXRows(N, K, "e2m1", DEV)
+    assert w.buffer.numel() > 1 << 31
+    w.buffer.random_(0, 256, generator=g)
+    w.buffer[-(-N // 16) * 32 * 1024:].random_(110, 130, generator=g)
+    small = tail(w, 4)
+    for M, kernel in ((3, "stream"), (70, "64x64"), (70, "256x128")):
+        a = made(numbers(M, K, M, 1), "e4m3")
+        out = torch.empty(M, N, dtype=torch.bfloat16, device=DEV)
+        ops.gemm_mx(out, a, w, kernel=kernel)
+        part = torch.empty(M, small.rows, dtype=torch.bfloat16, device=DEV)
+        ops.gemm_mx(part, a, small, kernel=kernel)
+        assert torch.equal(out[:, -small.rows:], part) and out.isfinite().all()
+        del out
+    # rows: 4.6 GB of numbers in, 2.4 GB of elements; and as many rows of a product
+    out = torch.empty(N, K, dtype=torch.bfloat16, device=DEV)
+    ops.mx_values(out, w)
+    part = torch.empty(small.rows, K, dtype=torch.bfloat16, device=DEV)
+    ops.mx_values(part, small)
+    assert torch.equal(out[-small.rows:], part)
+    again = ops.MXRows(N, K, "e2m1", DEV)
+    ops.mx_quantize(again, out)
+    part2 = torch.empty_like(part)
+    ops.mx_values(part2, tail(again, 4))
+    assert torch.equal(part2, part)      # (values of the format stay as they are)
+    narrow = made(numbers(130, K, 9, 1), "e2m1")
+    prod = torch.empty(N, 130, device=DEV)
+    ops.gemm_mx(prod, w, narrow)
+    few = torch.empty(small.rows, 130, device=DEV)
+    ops.gemm_mx(few, small, narrow, kernel="256x128")
+    assert (prod[-small.rows:] - few).abs().max() <= 1e-4 * few.abs().max()
 
 
 FORMS = [f for f in ops.MX_FORMS if f is not None]
