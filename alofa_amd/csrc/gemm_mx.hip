@@ -54,9 +54,10 @@ __device__ __forceinline__ f32x4 mx_multiply(const MxOperand<kE2M1>& w, const Mx
 }
 
 // ---- few rows: the matrix is streamed once -------------------------------------
-// A block computes NT tiles of 16 outputs for MT tiles of 16 rows. Its waves share out K tile by tile, every wave with two sets of U tiles of 128 on their way or under its products; the waves' sums
-// meet in LDS and are added in the waves' order. Lanes whose row lies behind the last one read the last one again: memory is asked for rows that there are only.
-template <int kAct, int NT, int MT, int kWaves, int U>
+// A block computes NT tiles of 16 outputs for MT tiles of 16 rows. Its waves share out K tile by tile, every wave with the next tile on its way under the products of one; the waves' sums meet in LDS and are
+// added in the waves' order. Lanes whose row lies behind the last one read the last one again: memory is asked for rows that there are only. What keeps memory busy is blocks side by side on a compute unit, not tiles
+// ahead: with two and three tiles a set, whose registers leave room for fewer blocks, 5,120 x 5,120 against 8 rows took 7.1 and 9.1 us (6.0), gate and up of 18,944 x 3,584 with eight waves a block 22.3 (17.2).
+template <int kAct, int NT, int MT, int kWaves>
 __device__ __forceinline__ void mx_stream(const MxMatrix& a, const MxMatrix (&w)[NT], const int (&w_tile)[NT], int M, int first_m_tile, int k_begin, int k_end, int k_tiles, f32x4 (&acc)[NT][MT]) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, shift = 8 * (lane / 16);
   int64_t a_tile[MT];
@@ -72,63 +73,49 @@ __device__ __forceinline__ void mx_stream(const MxMatrix& a, const MxMatrix (&w)
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   struct Set {
-    MxFragment<kE2M1> w[U][NT];
-    MxFragment<kAct> a[U][MT];
+    MxFragment<kE2M1> w[NT];
+    MxFragment<kAct> a[MT];
   };
-  // (every load is always made, so that the compiler can count them: behind the end of K the last tile again, whose elements of the matrix become zeros)
   auto load = [&](Set& s, int kt) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = min(kt + u * kWaves, k_end - 1);
+    for (int i = 0; i < NT; ++i) s.w[i].load(w[i], static_cast<int64_t>(w_tile[i]) * k_tiles + kt, lane);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) s.w[u][i].load(w[i], static_cast<int64_t>(w_tile[i]) * k_tiles + at, lane);
+    for (int j = 0; j < MT; ++j) s.a[j].load(a, a_tile[j] + kt, a_at[j]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&](const Set& s) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < MT; ++j) s.a[u][j].load(a, a_tile[j] + at, a_at[j]);
+    for (int j = 0; j < MT; ++j) {
+      const MxOperand<kAct> a_op(s.a[j], shift);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) acc[i][j] = mx_multiply<kAct>(MxOperand<kE2M1>(s.w[i], shift), a_op, acc[i][j]);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto multiply = [&](Set& s, int kt) __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t there = kt + u * kWaves < k_end ? ~0u : 0u;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        uint4& x = s.w[u][i].half[0];
-        x = make_uint4(x.x & there, x.y & there, x.z & there, x.w & there);
-      }
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const MxOperand<kAct> a_op(s.a[u][j], shift);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) acc[i][j] = mx_multiply<kAct>(MxOperand<kE2M1>(s.w[u][i], shift), a_op, acc[i][j]);
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  constexpr int kStep = kWaves * U;
   int kt = k_begin + wave;
   if (kt >= k_end) return;      // (uniform over the wave)
   Set s0, s1;
   load(s0, kt);
   while (true) {
-    if (kt + kStep >= k_end) {
-      multiply(s0, kt);
+    kt += kWaves;
+    if (kt >= k_end) {
+      multiply(s0);
       return;
     }
-    load(s1, kt + kStep);
-    multiply(s0, kt);
-    kt += 2 * kStep;
+    load(s1, kt);
+    multiply(s0);
+    kt += kWaves;
     if (kt >= k_end) {
-      multiply(s1, kt - kStep);
+      multiply(s1);
       return;
     }
     load(s0, kt);
-    multiply(s1, kt - kStep);
+    multiply(s1);
   }
 }
 
-template <typename TO, int kAct, int NT, int MT, int kWaves, int U>
-__global__ void __launch_bounds__(kWaves * kWave, MT == 1 ? 4 : 1) mx_stream_kernel(TO* __restrict__ out, int64_t ldo, int64_t share_stride, MxMatrix a, MxMatrix w, const float* __restrict__ bias, int M, int N,
+template <typename TO, int kAct, int NT, int MT, int kWaves>
+__global__ void __launch_bounds__(kWaves * kWave) mx_stream_kernel(TO* __restrict__ out, int64_t ldo, int64_t share_stride, MxMatrix a, MxMatrix w, const float* __restrict__ bias, int M, int N,
                                                                    int k_tiles, int epilogue, int vec) {
   __shared__ f32x4 sums[NT * MT][kWaves][kWave];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
@@ -139,7 +126,7 @@ __global__ void __launch_bounds__(kWaves * kWave, MT == 1 ? 4 : 1) mx_stream_ker
 #pragma unroll
   for (int i = 0; i < NT; ++i) ws[i] = w, tiles[i] = min(static_cast<int>(blockIdx.x) * NT + i, w.tiles - 1);
   f32x4 acc[NT][MT];
-  mx_stream<kAct, NT, MT, kWaves, U>(a, ws, tiles, M, blockIdx.y * MT, k_begin, k_end, k_tiles, acc);
+  mx_stream<kAct, NT, MT, kWaves>(a, ws, tiles, M, blockIdx.y * MT, k_begin, k_end, k_tiles, acc);
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -154,7 +141,7 @@ __global__ void __launch_bounds__(kWaves * kWave, MT == 1 ? 4 : 1) mx_stream_ker
 }
 
 // Gate and up of the same 32 outputs, act(gate) * up, one block of a microscaled row of the output.
-template <int kAct, int kOut, int MT, int kWaves, int U>
+template <int kAct, int kOut, int MT, int kWaves>
 __global__ void __launch_bounds__(kWaves * kWave) mx_stream_gated_kernel(uint8_t* __restrict__ out, int64_t out_scales_at, int out_tiles, MxMatrix a, MxMatrix gate, MxMatrix up, int M, int N,
                                                                          int k_tiles, int gelu) {
   __shared__ f32x4 sums[4][kWaves][kWave];
@@ -164,7 +151,7 @@ __global__ void __launch_bounds__(kWaves * kWave) mx_stream_gated_kernel(uint8_t
   const int t0 = min(2 * static_cast<int>(blockIdx.x), gate.tiles - 1), t1 = min(2 * static_cast<int>(blockIdx.x) + 1, gate.tiles - 1);
   const int tiles[4] = {t0, t1, t0, t1};
   f32x4 acc[4][MT];
-  mx_stream<kAct, 4, MT, kWaves, U>(a, ws, tiles, M, blockIdx.y * MT, 0, k_tiles, k_tiles, acc);
+  mx_stream<kAct, 4, MT, kWaves>(a, ws, tiles, M, blockIdx.y * MT, 0, k_tiles, k_tiles, acc);
   for (int j = 0; j < MT; ++j) {
     __syncthreads();
 #pragma unroll
@@ -296,8 +283,8 @@ static int product_shares(void* out, int dtype, int64_t ldo, int shares, int64_t
   // (as many tiles of the matrix as of rows: what is read of the rows, and e4m3 taken apart, serves them all)
   const int mt = stream_tiles(M);
   const dim3 grid((mw.tiles + mt - 1) / mt, (ma.tiles + mt - 1) / mt, shares);
-#define GO(T, ACT, MT, U) mx_stream_kernel<T, ACT, MT, MT, (MT == 4 ? 4 : 8), U><<<grid, (MT == 4 ? 256 : 512), 0, stream>>>(static_cast<T*>(out), ldo, share_stride, ma, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec)
-#define GO_MT(T, ACT) do { if (mt == 1) GO(T, ACT, 1, 3); else if (mt == 2) GO(T, ACT, 2, 2); else GO(T, ACT, 4, 1); } while (0)
+#define GO(T, ACT, MT) mx_stream_kernel<T, ACT, MT, MT, (MT == 4 ? 4 : 8)><<<grid, (MT == 4 ? 256 : 512), 0, stream>>>(static_cast<T*>(out), ldo, share_stride, ma, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec)
+#define GO_MT(T, ACT) do { if (mt == 1) GO(T, ACT, 1); else if (mt == 2) GO(T, ACT, 2); else GO(T, ACT, 4); } while (0)
   if (dtype == kF32) { if (a_kind == kE2M1) GO_MT(float, kE2M1); else GO_MT(float, kE4M3); }
   else { if (a_kind == kE2M1) GO_MT(bf16_t, kE2M1); else GO_MT(bf16_t, kE4M3); }
 #undef GO_MT
@@ -349,7 +336,7 @@ extern "C" int alofa_gemm_swiglu_mx(void* out, int out_kind, const void* a, int 
   if (form != kMxStream) return launch_mx_tiles_gated(form, static_cast<uint8_t*>(out), out_kind, at, out_tiles, ma, a_kind, mg, mu, static_cast<int>(M), static_cast<int>(N), k_tiles, gelu != 0, stream);
   const int mt = stream_tiles(M);
   const dim3 grid(4 * out_tiles, (ma.tiles + mt - 1) / mt);
-#define GO(ACT, OUT, MT) mx_stream_gated_kernel<ACT, OUT, MT, (MT == 4 ? 4 : 8), (MT == 1 ? 2 : 1)><<<grid, (MT == 4 ? 256 : 512), 0, stream>>>(static_cast<uint8_t*>(out), at, out_tiles, ma, mg, mu, static_cast<int>(M), static_cast<int>(N), k_tiles, gelu)
+#define GO(ACT, OUT, MT) mx_stream_gated_kernel<ACT, OUT, MT, 4><<<grid, 256, 0, stream>>>(static_cast<uint8_t*>(out), at, out_tiles, ma, mg, mu, static_cast<int>(M), static_cast<int>(N), k_tiles, gelu)
 #define GO_MT(ACT, OUT) do { if (mt == 1) GO(ACT, OUT, 1); else if (mt == 2) GO(ACT, OUT, 2); else GO(ACT, OUT, 4); } while (0)
   if (a_kind == kE2M1) { if (out_kind == kE2M1) GO_MT(kE2M1, kE2M1); else GO_MT(kE2M1, kE4M3); }
   else { if (out_kind == kE2M1) GO_MT(kE4M3, kE2M1); else GO_MT(kE4M3, kE4M3); }
