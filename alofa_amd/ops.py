@@ -77,11 +77,7 @@ _scope = _Scope()      # (a thread's own, as torch's current stream is)
 def _stream() -> int:
     if _scope.stream is not None:
         return _scope.stream
-    return _current_stream(torch.cuda.current_device())
-
-
-# torch's current stream of a device as the launches take it: its own way to that number where it has one (0.4 us with the device's number; by way of a Stream object 2.7)
-_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+    return torch.cuda.current_stream().cuda_stream
 
 
 class stream_scope:
@@ -2874,6 +2870,16 @@ def _out_rows(name: str, t: torch.Tensor) -> int:
     return ld
 
 
+# torch's current stream of a device as the launches take it: its own way to that number where it has one (0.4 us with the device's number; by way of a Stream object 2.7)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _stream_on(device: int) -> int:
+    """``_stream`` where that device is known to be the current one."""
+    stream = _scope.stream
+    return _current_stream(device) if stream is None else stream
+
+
 _here = torch.cuda.current_device      # (the kernels go to the current device's stream)
 
 
@@ -2889,7 +2895,7 @@ def mx_quantize(out: MXRows, x: torch.Tensor) -> None:
     """The nearest microscaled rows to ``x`` [rows, k] (float32 or bfloat16, rows contiguous). A block's scale is the smallest power of two under which its largest magnitude is at
     most half a step beyond the largest element (7 for e2m1, 464 for e4m3), 2^-127 at least; its elements are rounded to the nearest, ties to even. A block with an infinity or a NaN is NaN throughout."""
     if type(out) is MXRows and _here() == out.device and (sizes := _native().mx_matrix(x, None, out.rows, out.k, out.device, 0)) is not None:
-        _call("alofa_mx_quantize", out.buffer, out.number, x, *sizes, out.rows, out.k, _stream())
+        _call("alofa_mx_quantize", out.buffer, out.number, x, *sizes, out.rows, out.k, _stream_on(out.device))
         return
     kind = _mx("out", out)
     _gpu("x", x, None, 2)
@@ -2903,7 +2909,7 @@ def mx_quantize(out: MXRows, x: torch.Tensor) -> None:
 def mx_values(out: torch.Tensor, q: MXRows) -> None:
     """out [rows, k] (float32, or bfloat16 rounded to the nearest) = the values that ``q`` stands for."""
     if type(q) is MXRows and _here() == q.device and (sizes := _native().mx_matrix(out, None, q.rows, q.k, q.device, 1)) is not None:
-        _call("alofa_mx_values", out, *sizes, q.buffer, q.number, q.rows, q.k, _stream())
+        _call("alofa_mx_values", out, *sizes, q.buffer, q.number, q.rows, q.k, _stream_on(q.device))
         return
     kind = _mx("q", q)
     _gpu("out", out, None, 2)
@@ -2937,7 +2943,7 @@ def rmsnorm_mx(out: MXRows, x: torch.Tensor, w: torch.Tensor, eps: float, add: O
     not depend on anything but the row."""
     if type(out) is MXRows and eps > 0 and _here() == out.device and (sizes := _native().mx_norm(x, w, add, total, out.rows, out.k, out.device)) is not None:
         ldx, shares, stride, ld_add, ld_total = sizes
-        _call("alofa_rmsnorm_mx", out.buffer, out.number, x, ldx, add, shares, stride, ld_add, total, ld_total, w, _F(eps), out.rows, out.k, _stream())
+        _call("alofa_rmsnorm_mx", out.buffer, out.number, x, ldx, add, shares, stride, ld_add, total, ld_total, w, _F(eps), out.rows, out.k, _stream_on(out.device))
         return
     kind = _mx("out", out)
     _gpu("x", x, torch.float32, 2), _contig("w", _gpu("w", w, torch.float32, 1))
@@ -2992,7 +2998,7 @@ def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor
     if _here() == a.device == w.device and (sizes := _native().mx_matrix(out, bias, M, N, a.device, 1)) is not None and (not add_to_out or (bias is None and sizes[0] == F32)):
         if shares > 1:
             parts = torch.empty(shares * M * N, dtype=torch.float32, device=out.device) if scratch is None else scratch("mx_sums", (shares * M * N,), torch.float32)
-        _call("alofa_gemm_mx", out, *sizes, shares, parts, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, form, _stream())
+        _call("alofa_gemm_mx", out, *sizes, shares, parts, a.buffer, kind, w.buffer, bias, M, N, K, ADD_TO_RESIDUAL if add_to_out else STORE, form, _stream_on(a.device))
         return
     _gpu("out", out, None, 2)
     if tuple(out.shape) != (M, N):
@@ -3038,5 +3044,6 @@ def gemm_swiglu_mx(out: MXRows, a: MXRows, w_gate: MXRows, w_up: MXRows, act: st
     out_kind = _mx("out", out)
     if w_up.rows != N or (out.rows, out.k) != (M, N):
         raise AlofaError("shape_mismatch", "gate/up product shapes do not fit", f"a={a} gate={w_gate} up={w_up} out={out}")
-    _one_device(out.buffer, a.buffer, w_gate.buffer, w_up.buffer)
-    _call("alofa_gemm_swiglu_mx", out.buffer, out_kind, a.buffer, kind, w_gate.buffer, w_up.buffer, M, N, K, int(act == "gelu_tanh"), _mx_form(kernel), _stream())
+    if not _here() == a.device == w_gate.device == w_up.device == out.device:
+        _one_device(out.buffer, a.buffer, w_gate.buffer, w_up.buffer)
+    _call("alofa_gemm_swiglu_mx", out.buffer, out_kind, a.buffer, kind, w_gate.buffer, w_up.buffer, M, N, K, int(act == "gelu_tanh"), _mx_form(kernel), _stream_on(a.device))
