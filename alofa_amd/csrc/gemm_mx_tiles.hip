@@ -19,8 +19,15 @@ struct MxTile {
   static_assert((BN + BM) / 64 <= kWaves, "a wave brings the scales of four tiles at most");
   static constexpr int kLoads = (kPieces + kWaves - 1) / kWaves + 1;    // a wave's, per slab (a wave with a piece less brings its first one again)
   static constexpr int kScales = kPieces * 1024, kSlab = kScales + kWaves * 256;
-  static_assert(S * kSlab <= 160 * 1024, "the ring fits LDS");
+  static_assert(S >= 2 && S * kSlab <= 160 * 1024 && (S - 2) * kLoads < 64, "the ring fits LDS, what is on its way is counted");
 };
+
+// A wave's loads of a slab have come, and its reads from LDS; those of `behind` slabs behind it, kMost at most, stay on their way.
+template <int kMost, int kLoads>
+__device__ __forceinline__ void wait_for(int behind) {
+  if (behind >= kMost) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(kMost * kLoads) : "memory");
+  else if constexpr (kMost > 0) wait_for<kMost - 1, kLoads>(behind);
+}
 
 // What a wave multiplies: acc[i][j] of the matrix's i-th 32 rows and the activations' j-th. `gated`: the first half of a wave's 32-row groups is the gate's, the second the same outputs' of up.
 template <int kAct, typename T, bool kGated>
@@ -154,9 +161,7 @@ __device__ __forceinline__ void mx_tile_product(char* ring, const MxMatrix a, co
     }
   for (int k = k_begin; k < k_end; ++k) {
     const int behind = k_end - 1 - k;
-    if (S > 2 && behind >= S - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((S - 2) * kLoads) : "memory");
-    else if (S == 4 && behind == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(kLoads) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    wait_for<S - 2, kLoads>(behind);
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
