@@ -307,6 +307,7 @@ extern "C" int alofa_rmsnorm_mx(void* out, int kind, const float* x, int64_t ldx
   if (!sizes_fit("rmsnorm_mx", kind, rows, k)) return 1;
   ALOFA_REQUIRE(out && x && w && aligned16(out) && shares >= 0 && (shares == 0 || add) && (shares == 0 || total) && ldx >= 0 && ld_add >= 0 && share_stride >= 0 && ld_total >= 0 && eps > 0.f,
                 "rmsnorm_mx: operands do not fit: shares=%d eps=%g", shares, static_cast<double>(eps));
+  ALOFA_REQUIRE(rows < 1 << 24, "rmsnorm_mx: more rows than a launch takes: %lld", static_cast<long long>(rows));
   const int k_tiles = static_cast<int>(mx_tiles(k, 128)), n = static_cast<int>(k);
   const int64_t at = mx_scales_at(rows, k, kind);
   const bool vec = k % 8 == 0 && aligned16(x) && ldx % 4 == 0 && aligned16(w) && (shares == 0 || (aligned16(add) && ld_add % 4 == 0 && share_stride % 4 == 0)) && (!total || (aligned16(total) && ld_total % 4 == 0));

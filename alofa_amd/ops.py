@@ -2993,7 +2993,7 @@ def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor
     form, shares, parts = -1, 1, None
     if kernel is not None:
         form = _mx_form(kernel)
-    elif M > 16 or K > 8192:
+    elif M > 16 or K > 8192:      # (the rule shares no smaller sum out: adding the shares up takes longer than the whole sum)
         shares = _answer("alofa_gemm_mx_shares", M, N, K, kind, 0)
     if _here() == a.device == w.device and (sizes := _native().mx_matrix(out, bias, M, N, a.device, 1)) is not None and (not add_to_out or (bias is None and sizes[0] == F32)):
         if shares > 1:
@@ -3020,6 +3020,11 @@ def gemm_mx(out: torch.Tensor, a: MXRows, w: MXRows, bias: Optional[torch.Tensor
 
 def mx_shares(M: int, N: int, K: int, kind: str = "e4m3") -> int:
     """Into how many shares of K the product of so many rows of ``kind`` with an [N, K] matrix is best cut where ``rmsnorm_mx`` adds them up."""
+    for name, n in (("M", M), ("N", N), ("K", K)):
+        if not 1 <= operator.index(n) <= 1 << 24:
+            raise AlofaError("shape_mismatch", "a product's sizes are 1 to 2^24", f"{name}={n}")
+    if kind not in MX_KINDS:
+        raise AlofaError("unsupported", "no such kind of microscaled element", f"kind={kind} known={','.join(MX_KINDS)}")
     return _answer("alofa_gemm_mx_shares", M, N, K, MX_KINDS[kind], 1)
 
 

@@ -75,12 +75,12 @@ def linear_params_per_layer(c):
     return h * (qd + 2 * kvd) + qd * h + 3 * h * i
 
 
-def decode_bytes(c, ctx_lens, dtype_bytes=2):
+def decode_bytes(c, ctx_lens, dtype_bytes=2, matrix_bytes=None):
     """Bytes one decode step has to read: every weight it uses once (layer
-    matrices, biases, norms, the output matrix) and the cache of the live requests."""
+    matrices, of ``matrix_bytes`` a number where that differs, biases, norms, the output matrix) and the cache of the live requests."""
     h, d, L = c["hidden_size"], c["hidden_size"] // c["num_attention_heads"], c["num_hidden_layers"]
     qd, kvd = c["num_attention_heads"] * d, c["num_key_value_heads"] * d
-    per_layer = linear_params_per_layer(c) * dtype_bytes + (qd + 2 * kvd) * 4 + 2 * h * 4
+    per_layer = linear_params_per_layer(c) * (matrix_bytes or dtype_bytes) + (qd + 2 * kvd) * 4 + 2 * h * 4
     weights = L * per_layer + h * 4 + c["vocab_size"] * h * dtype_bytes
     cache = sum(ctx_lens) * 2 * kvd * dtype_bytes * L
     return weights + cache
@@ -209,14 +209,17 @@ def spread(samples):
             "max_ms": round(max(samples) * 1e3, 4), "repeats": len(samples)}
 
 
-def device_model(cfg, dtype, seed):
-    """(config, model) with random weights drawn on the device: for sizes whose file would take minutes to write."""
+def device_model(cfg, dtype, seed, matrices="stored"):
+    """(config, model) with random weights drawn on the device: for sizes whose file would take minutes to write. ``matrices``: as for ``load_model``."""
     import torch
     from alofa_amd.config import config_from_dict
     from alofa_amd.model import Model, expected_tensors, runtime
     from alofa_amd.weights import random_tensors
     config = config_from_dict(cfg)
     spec = config.spec()
+    if matrices == "mxfp4":
+        from alofa_amd.parts.microscaled import microscaled
+        spec = microscaled(spec)
     rt = runtime(dtype)
     weights = random_tensors(expected_tensors(spec), seed, device=rt.device)
     model = Model(spec, weights, rt)
@@ -472,12 +475,22 @@ def long_prompts(args):
 
 def sweep(args):
     """Decode steps over batch sizes (at a context of about 550) or over contexts (batch 1, 8, 32): one line per
-    point with ms per step, tokens a second and the bytes the step has to read / time. At the 0.5B sizes, or with
-    --config 1.5b .. 32b at those (batches up to 64; --layers for fewer layers than the configuration has)."""
+    point with ms per step, tokens a second and the bytes the step has to read / time; or one prompt of 512, 2,048 and 8,192
+    tokens. At the 0.5B sizes, or with --config 1.5b .. 32b at those (batches up to 64; --layers for fewer layers than the
+    configuration has). With --matrices mxfp4 the layers' matrices are held in 4 bits."""
     name = args.config
     cfg = dict(CONFIGS[name], num_hidden_layers=args.layers or CONFIGS[name]["num_hidden_layers"])
-    model = device_model(cfg, args.dtype, 20260918)
+    model = device_model(cfg, args.dtype, 20260918, args.matrices)
     dbytes = 2 if args.dtype == "bfloat16" else 4
+    mbytes, which = (17 / 32, {"matrices": "mxfp4"}) if args.matrices == "mxfp4" else (None, {})
+    if args.sweep == "prefill":
+        for T in (512, 2048, 8192) if args.prompt == PROMPT else (args.prompt,):
+            p = PrefillPoint(model, cfg, args.dtype, T)
+            p.run()
+            s = min(p.run() for _ in range(3))
+            print(json.dumps({"model": name, **which, "layers": cfg["num_hidden_layers"], "prompt": T, "ms": round(s * 1e3, 3), "tok_s": round(T / s, 1),
+                              "tflops": round(prefill_flops(cfg, T) / s / 1e12, 1)}), flush=True)
+        return 0
     batches = (1, 2, 4, 8, 16, 17, 24, 32, 48, 64, 96, 128, 192, 256) if name == "0.5b" else (1, 2, 4, 8, 16, 17, 32, 64) if name in ("1.5b", "3b") else (1, 2, 4, 8, 16, 32, 64)
     if args.batches:
         batches = tuple(int(b) for b in args.batches.split(","))
@@ -487,8 +500,8 @@ def sweep(args):
         pt = DecodePoint(model, cfg, args.dtype, batch, prompt, context=max(CONTEXT, prompt + 256))
         pt.run(8)
         s = pt.run(24)
-        byts = decode_bytes(cfg, pt.context_lengths(), dbytes)
-        print(json.dumps({"model": name, "layers": cfg["num_hidden_layers"], "batch": batch, "context": prompt, "ms_per_step": round(s * 1e3, 4), "tok_s": round(batch / s, 1),
+        byts = decode_bytes(cfg, pt.context_lengths(), dbytes, mbytes)
+        print(json.dumps({"model": name, **which, "layers": cfg["num_hidden_layers"], "batch": batch, "context": prompt, "ms_per_step": round(s * 1e3, 4), "tok_s": round(batch / s, 1),
                           "gb_s": round(byts / s / 1e9, 1), "frac_hbm": round(byts / s / 1e9 / PEAK_HBM_GBS, 4)}), flush=True)
         pt.close()
     return 0
@@ -652,13 +665,17 @@ def main():
     ap.add_argument("--only-prefill", action="store_true", help="run the 2,048-token prefill alone (for profiling) and print its line")
     ap.add_argument("--serve", action="store_true", help="the continuous batch of 64 requests (prompts of 128..2,048 tokens, 256 new tokens, chunks of 512) at the sizes of --config")
     ap.add_argument("--batches", default=None, help="with --sweep batch: these batch sizes only (comma-separated), e.g. to profile one point")
-    ap.add_argument("--sweep", choices=["batch", "context"], default=None, help="decode steps over batch sizes or over contexts, a line per point (the sizes of --config)")
+    ap.add_argument("--sweep", choices=["batch", "context", "prefill"], default=None, help="decode steps over batch sizes or over contexts, or one prompt's prefill, a line per point (the sizes of --config)")
+    ap.add_argument("--matrices", choices=["stored", "mxfp4"], default="stored", help="with --sweep: mxfp4: the layers' matrices in 4 bits (with bfloat16)")
     ap.add_argument("--design", choices=sorted(DESIGN_MODELS), default=None, help="prefill and decode of this design beside the closest one at equal sizes (--sizes), a line per point")
     ap.add_argument("--sizes", default=None, help=f"with --design: which of {','.join(DESIGN_SIZES)} (comma-separated; default {','.join(DESIGN_DEFAULT)})")
     ap.add_argument("--only", choices=sorted(DESIGN_MODELS) + ["qwen2"], default=None, help="with --design: this model alone (for profiling)")
     ap.add_argument("--prompt-tokens", type=int, default=2048, help="with --design: tokens of the prefill point's prompt")
     ap.add_argument("--no-prefill", action="store_true", help="with --design: decode points only")
     args = ap.parse_args()
+    if args.matrices != "stored" and not args.sweep:
+        print("--matrices goes with --sweep")
+        return 2
     if args.gpus != 1:
         print("bench.py measures one GPU only: this engine has no multi-GPU path (--gpus must be 1)")
         return 2

@@ -98,3 +98,9 @@ def test_an_engine_over_a_given_model_does_not_change_its_matrices():
     from alofa_amd import Engine
     with pytest.raises(AlofaError):
         Engine(None, model=(None, None), matrices="mxfp4")
+
+
+@pytest.mark.parametrize("M,N,K,kind", [(0, 32, 64, "e4m3"), (4, -1, 64, "e4m3"), (4, 32, 0, "e2m1"), (4, 32, 1 << 25, "e2m1"), (1 << 25, 32, 64, "e4m3"), (4, 32, 64, "e5m2")])
+def test_shares_of_sizes_and_kinds_that_are_refused(M, N, K, kind):
+    with pytest.raises(AlofaError):
+        ops.mx_shares(M, N, K, kind)

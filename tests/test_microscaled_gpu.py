@@ -507,3 +507,13 @@ def test_refusals():
             pytest.fail(f"call {k} was not refused")
     ops.gemm_mx(out, a, w)      # (and what is left as it was still runs)
     torch.cuda.synchronize()
+
+
+def test_more_rows_than_a_norms_launch_takes_are_refused():
+    rows = 1 << 24      # (a block of 256 threads each: 2^32 threads)
+    out = ops.MXRows(rows, 32, "e2m1", DEV)
+    out.buffer[:64].zero_()
+    with pytest.raises(AlofaError):
+        ops.rmsnorm_mx(out, torch.ones(1, 32, device=DEV).expand(rows, 32), torch.ones(32, device=DEV), 1e-6)
+    torch.cuda.synchronize()
+    assert not out.buffer[:64].any()
