@@ -46,17 +46,13 @@ struct MxOperand {
   }
 };
 
-template <int kAct>
-__device__ __forceinline__ f32x4 mx_multiply(const MxOperand<kE2M1>& w, const MxOperand<kAct>& a, f32x4 acc) {
-  acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.part[0], a.part[0], acc, kE2M1, kAct, 0, w.scale, 0, a.scale);
-  if constexpr (kAct == kE4M3) acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.part[0], a.part[1], acc, kE2M1, kAct, 0, w.scale, 0, a.scale);
-  return acc;
-}
-
 // ---- few rows: the matrix is streamed once -------------------------------------
-// A block computes NT tiles of 16 outputs for MT tiles of 16 rows. Its waves share out K tile by tile, every wave with the next tile on its way under the products of one; the waves' sums meet in LDS and are
-// added in the waves' order. Lanes whose row lies behind the last one read the last one again: memory is asked for rows that there are only. What keeps memory busy is blocks side by side on a compute unit, not tiles
-// ahead: with two and three tiles a set, whose registers leave room for fewer blocks, 5,120 x 5,120 against 8 rows took 7.1 and 9.1 us (6.0), gate and up of 18,944 x 3,584 with eight waves a block 22.3 (17.2).
+// A block computes NT tiles of 16 outputs for MT tiles of 16 rows. Its waves share out K tile by tile, every wave with the next tile of the matrix on its way under the products of one; the waves' sums meet in LDS and are
+// added in the waves' order. Nothing is waited for together but at the end. Lanes whose row lies behind the last one read the last one again: memory is asked for rows that there are only.
+// Up to 16 rows memory bounds it: gate and up of 18,944 x 3,584 take 16.6 us (4.3 TB/s; 27,648 x 5,120 30.7, 4.9), 3,584 x 18,944 11.3, 7,168 x 5,120 6.6. What keeps it busy is waves side by side, not tiles ahead: with
+// two and three tiles a set, whose registers leave room for fewer, 5,120 x 5,120 against 8 rows took 7.1 and 9.1 us (6.0), gate and up with eight waves a block 22.3.
+// With more rows it is what the caches give, 13 TB/s over all compute units (333 rows against 18,944 x 3,584 by 4 x 4 tiles: 622 MB in 50 us); so rows and matrix are taken by equal numbers of tiles where blocks are many. Where
+// they are few, 2 x 4 tiles and eight waves keep more compute units busy: 64 rows against 4,608 x 3,584 take 7.6 us (4 x 4: 10.1; 1 x 4: 11.0), against 18,944 x 3,584 22.1 (18.2).
 template <int kAct, int NT, int MT, int kWaves>
 __device__ __forceinline__ void mx_stream(const MxMatrix& a, const MxMatrix (&w)[NT], const int (&w_tile)[NT], int M, int first_m_tile, int k_begin, int k_end, int k_tiles, f32x4 (&acc)[NT][MT]) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, shift = 8 * (lane / 16);
@@ -72,50 +68,51 @@ __device__ __forceinline__ void mx_stream(const MxMatrix& a, const MxMatrix (&w)
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  struct Set {
-    MxFragment<kE2M1> w[NT];
-    MxFragment<kAct> a[MT];
-  };
-  auto load = [&](Set& s, int kt) __attribute__((always_inline)) {
+  // Two sets of the matrix's fragments, one of the rows': a tile of rows is asked for anew as soon as its registers are free, i.e. taken into the instruction's operands.
+  typedef MxFragment<kE2M1> Matrix[NT];
+  Matrix w0, w1;
+  MxFragment<kAct> rows[MT];
+  auto load = [&](Matrix& f, int kt) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) s.w[i].load(w[i], static_cast<int64_t>(w_tile[i]) * k_tiles + kt, lane);
-#pragma unroll
-    for (int j = 0; j < MT; ++j) s.a[j].load(a, a_tile[j] + kt, a_at[j]);
+    for (int i = 0; i < NT; ++i) f[i].load(w[i], static_cast<int64_t>(w_tile[i]) * k_tiles + kt, lane);
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto multiply = [&](const Set& s) __attribute__((always_inline)) {
+  auto multiply = [&](const Matrix& f, auto more, int next) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
-      const MxOperand<kAct> a_op(s.a[j], shift);
+      const MxOperand<kAct> a_op(rows[j], shift);
+      if constexpr (decltype(more)::value) {
+        rows[j].load(a, a_tile[j] + next, a_at[j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
-      for (int i = 0; i < NT; ++i) acc[i][j] = mx_multiply<kAct>(MxOperand<kE2M1>(s.w[i], shift), a_op, acc[i][j]);
+      for (int part = 0; part < (kAct == kE2M1 ? 1 : 2); ++part)      // (an instruction whose sums are those of the one before it waits for them)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const MxOperand<kE2M1> w_op(f[i], shift);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w_op.part[0], a_op.part[part], acc[i][j], kE2M1, kAct, 0, w_op.scale, 0, a_op.scale);
+        }
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  int kt = k_begin + wave;
-  if (kt >= k_end) return;      // (uniform over the wave)
-  Set s0, s1;
-  load(s0, kt);
-  while (true) {
-    kt += kWaves;
-    if (kt >= k_end) {
-      multiply(s0);
-      return;
-    }
-    load(s1, kt);
-    multiply(s0);
-    kt += kWaves;
-    if (kt >= k_end) {
-      multiply(s1);
-      return;
-    }
-    load(s0, kt);
-    multiply(s1);
+  const int first = k_begin + wave, last = k_end - 1 - (k_end - 1 - first) % kWaves;      // this wave's tiles: first, first + kWaves, .., last
+  if (first >= k_end) return;      // (uniform over the wave)
+#pragma unroll
+  for (int j = 0; j < MT; ++j) rows[j].load(a, a_tile[j] + first, a_at[j]);
+  load(w0, first);
+  int kt = first;
+  for (; kt < last; kt += 2 * kWaves) {      // (behind an even number of tiles the last one is asked for again: a branch around the loads would have the compiler wait for all that are on their way)
+    const int after = min(kt + 2 * kWaves, last);
+    load(w1, kt + kWaves);
+    multiply(w0, std::true_type{}, kt + kWaves);
+    load(w0, after);
+    multiply(w1, std::true_type{}, after);
   }
+  if (kt == last) multiply(w0, std::false_type{}, 0);
 }
 
 template <typename TO, int kAct, int NT, int MT, int kWaves>
-__global__ void __launch_bounds__(kWaves * kWave) mx_stream_kernel(TO* __restrict__ out, int64_t ldo, int64_t share_stride, MxMatrix a, MxMatrix w, const float* __restrict__ bias, int M, int N,
+__global__ void __launch_bounds__(kWaves * kWave, MT == 4 ? 2 : 3) mx_stream_kernel(TO* __restrict__ out, int64_t ldo, int64_t share_stride, MxMatrix a, MxMatrix w, const float* __restrict__ bias, int M, int N,
                                                                    int k_tiles, int epilogue, int vec) {
   __shared__ f32x4 sums[NT * MT][kWaves][kWave];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
@@ -142,7 +139,7 @@ __global__ void __launch_bounds__(kWaves * kWave) mx_stream_kernel(TO* __restric
 
 // Gate and up of the same 32 outputs, act(gate) * up, one block of a microscaled row of the output.
 template <int kAct, int kOut, int MT, int kWaves>
-__global__ void __launch_bounds__(kWaves * kWave) mx_stream_gated_kernel(uint8_t* __restrict__ out, int64_t out_scales_at, int out_tiles, MxMatrix a, MxMatrix gate, MxMatrix up, int M, int N,
+__global__ void __launch_bounds__(kWaves * kWave, MT == 2 ? 2 : 4) mx_stream_gated_kernel(uint8_t* __restrict__ out, int64_t out_scales_at, int out_tiles, MxMatrix a, MxMatrix gate, MxMatrix up, int M, int N,
                                                                          int k_tiles, int gelu) {
   __shared__ f32x4 sums[4][kWaves][kWave];
   __shared__ float acts[16][36];
@@ -224,42 +221,54 @@ __global__ void __launch_bounds__(256) mx_sum_kernel(TO* __restrict__ out, int64
   mx_store4(out, ldo, bias, m, n, M, N, v, epilogue, vec != 0);
 }
 
-// What a product takes in each form, in us as measured, and how it is chosen. Tiles: a slab of 128 where a compute unit has one block, where it has several (each), and besides the slabs (64 to 1,024 blocks
-// of 16 and 48 slabs). The streaming kernel: a tile of 128 along K of a wave, for one, two and four tiles of rows (and of the matrix). A sum that is shared out over K takes a launch more, which adds the shares up, unless a norm does.
+// What a product takes in each form, in us, and how it is chosen: besides + more (each - 1) + turns max(alone, each * of_each), where a compute unit has `each` blocks and a block takes `step` slabs of 128 along K in a
+// turn. Fitted to 1,200 measured products (1 to 2,048 rows, matrices of 1,152 x 896 to 18,944 x 3,584 and 3,584 x 18,944; 3 % off in the mean with e4m3, 6 % with e2m1). Read along a column: tiles of 256 x 256 pay where all
+// compute units have some, small ones and the streaming kernel where blocks are few: 333 rows against 4,608 x 3,584 take 15.5 us by 64 x 64 streamed, 16.8 and 17.8 by tiles of 64 x 64 and 64 x 128, 25.4 by 128 x 128 and 41 by
+// 256 x 128; 700 rows against 18,944 x 3,584 91, 94, 80 and 85. A sum that is shared out over K takes a launch more, which adds the shares up, unless a norm does.
 struct MxCost {
-  int form, rows, columns;
-  float alone, each, besides;
+  int form, rows, columns, step;
+  float alone, of_each, besides, more;
 };
-constexpr MxCost kMxRows8[] = {{kMx256x256, 256, 256, 2.58f, 2.58f, 11.f}, {kMx256x192, 256, 192, 2.05f, 2.05f, 9.f},  {kMx256x160, 256, 160, 1.85f, 1.78f, 8.f}, {kMx256x128, 256, 128, 1.48f, 1.44f, 7.5f},
-                               {kMx128x128, 128, 128, 0.86f, 0.71f, 5.8f}, {kMx128x64, 128, 64, 0.60f, 0.44f, 5.f}, {kMx64x128, 64, 128, 0.60f, 0.44f, 5.f}, {kMx64x64, 64, 64, 0.57f, 0.31f, 5.f}};
-constexpr MxCost kMxRows4[] = {{kMx256x256, 256, 256, 0.99f, 0.99f, 9.5f}, {kMx256x192, 256, 192, 0.82f, 0.83f, 8.5f}, {kMx256x160, 256, 160, 0.72f, 0.74f, 8.f}, {kMx256x128, 256, 128, 0.58f, 0.53f, 7.f},
-                               {kMx128x128, 128, 128, 0.40f, 0.30f, 6.f}, {kMx128x64, 128, 64, 0.27f, 0.17f, 5.f}, {kMx64x128, 64, 128, 0.27f, 0.17f, 5.f}, {kMx64x64, 64, 64, 0.21f, 0.10f, 5.f}};
-constexpr int kMxStreamRows = 256;      // most rows that the streaming kernel is asked for
+constexpr MxCost kMxTiles8[] = {{kMx256x256, 256, 256, 1, 2.31f, 2.31f, 7.9f, 9.7f},  {kMx256x192, 256, 192, 1, 1.87f, 1.87f, 6.6f, 5.8f}, {kMx256x160, 256, 160, 1, 1.63f, 1.63f, 6.5f, 7.8f},
+                                {kMx256x128, 256, 128, 1, 1.35f, 1.35f, 5.5f, 4.3f},  {kMx128x128, 128, 128, 1, 0.76f, 0.65f, 5.3f, 1.6f}, {kMx128x64, 128, 64, 1, 0.52f, 0.43f, 4.2f, 0.8f},
+                                {kMx64x128, 64, 128, 1, 0.48f, 0.42f, 4.4f, 0.9f},    {kMx64x64, 64, 64, 1, 0.35f, 0.22f, 4.2f, 0.5f}};
+constexpr MxCost kMxTiles4[] = {{kMx256x256, 256, 256, 1, 0.82f, 0.82f, 7.8f, 10.2f}, {kMx256x192, 256, 192, 1, 0.73f, 0.74f, 6.1f, 5.5f}, {kMx256x160, 256, 160, 1, 0.61f, 0.61f, 6.5f, 9.3f},
+                                {kMx256x128, 256, 128, 1, 0.55f, 0.51f, 5.2f, 1.5f},  {kMx128x128, 128, 128, 1, 0.34f, 0.31f, 5.3f, 1.2f}, {kMx128x64, 128, 64, 1, 0.25f, 0.21f, 4.1f, 0.5f},
+                                {kMx64x128, 64, 128, 1, 0.25f, 0.22f, 4.3f, 0.8f},    {kMx64x64, 64, 64, 1, 0.19f, 0.12f, 4.2f, 0.3f}};
+// The streaming kernel: for one, two and four tiles of rows, and for one and two with a gate (columns of gate and up together); four by four
+constexpr MxCost kMxStream8[] = {{kMxStream, 16, 16, 8, 0.4f, 0.4f, 4.3f, 0.f}, {kMxStream, 32, 32, 8, 0.75f, 0.75f, 4.3f, 0.f}, {kMxStream, 64, 32, 8, 1.09f, 1.09f, 4.3f, 1.5f},
+                                 {kMxStream, 16, 64, 4, 0.6f, 0.6f, 4.3f, 0.f}, {kMxStream, 32, 64, 4, 0.59f, 0.59f, 4.3f, 0.4f}};
+constexpr MxCost kMxStream4[] = {{kMxStream, 16, 16, 8, 0.25f, 0.25f, 4.3f, 0.f}, {kMxStream, 32, 32, 8, 0.45f, 0.45f, 4.3f, 0.f}, {kMxStream, 64, 32, 8, 0.47f, 0.47f, 4.3f, 0.5f},
+                                 {kMxStream, 16, 64, 4, 0.55f, 0.55f, 4.3f, 0.f}, {kMxStream, 32, 64, 4, 0.55f, 0.55f, 4.3f, 0.f}};
+constexpr MxCost kMxWide8 = {kMxStream64x64, 64, 64, 4, 0.87f, 0.77f, 4.3f, 1.1f}, kMxWide4 = {kMxStream64x64, 64, 64, 4, 0.45f, 0.36f, 4.3f, 1.5f};
+constexpr int kMxStreamRows = 512;      // most rows that the streaming kernel is asked for (the largest products measured with it)
 
 struct MxPlan {
   int form, shares;
   float us;
 };
 
-static int stream_tiles(int64_t M) { return M > 32 ? 4 : M > 16 ? 2 : 1; }
+// tiles of rows that a block of the streaming kernel takes
+static int stream_tiles(int64_t M, bool gated) { return M > 32 && !gated ? 4 : M > 16 ? 2 : 1; }
 
 // The quickest form for so many shares
 static MxPlan plan_for(int64_t M, int64_t N, int k_tiles, int kind, bool gated, int shares) {
   MxPlan best = {kMx64x64, shares, 0.f};
   const int64_t units = compute_units(), slabs = mx_tiles(k_tiles, shares);
+  auto consider = [&](const MxCost& c) {
+    const int64_t blocks = mx_tiles(M, c.rows) * mx_tiles(N, c.columns) * shares;
+    const float each = static_cast<float>(mx_tiles(blocks, units)), us = c.besides + c.more * (each - 1.f) + static_cast<float>(mx_tiles(slabs, c.step)) * fmaxf(c.alone, each * c.of_each);
+    if (best.us == 0.f || us < best.us) best = {c.form, shares, us};
+  };
+  const bool few = kind == kE2M1;
   if (M <= kMxStreamRows) {
-    const int mt = stream_tiles(M), waves = mt == 4 ? 4 : 8;
-    const int64_t blocks = mx_tiles(M, 16 * mt) * (gated ? mx_tiles(N, 64) : mx_tiles(N, 16 * mt)) * shares;
-    const float tile = gated ? (mt == 4 ? 1.9f : mt == 2 ? 1.8f : 1.4f) : mt == 4 ? 1.0f : mt == 2 ? 0.85f : 0.42f;
-    best = {kMxStream, shares, 4.5f + (kind == kE2M1 ? 0.6f : 1.f) * tile * static_cast<float>(mx_tiles(slabs, waves)) * static_cast<float>(mx_tiles(blocks, units))};
+    const int mt = stream_tiles(M, gated), which = (gated ? 3 : 0) + mt / 2;
+    consider(few ? kMxStream4[which] : kMxStream8[which]);
+    if (mt == 4) consider(few ? kMxWide4 : kMxWide8);
   }
   if (M > 16)
-    for (const MxCost& c : kind == kE2M1 ? kMxRows4 : kMxRows8) {
-      if (gated && c.form == kMx256x160) continue;
-      const int64_t blocks = mx_tiles(M, c.rows) * mx_tiles(N, c.columns) * shares, each = mx_tiles(blocks, units);
-      const float us = c.besides + 3.f * static_cast<float>(each - 1) + static_cast<float>(slabs) * fmaxf(c.alone, static_cast<float>(each) * c.each);
-      if (best.us == 0.f || us < best.us) best = {c.form, shares, us};
-    }
+    for (const MxCost& c : few ? kMxTiles4 : kMxTiles8)
+      if (!gated || c.form != kMx256x160) consider(c);
   return best;
 }
 
@@ -279,15 +288,14 @@ static int product_shares(void* out, int dtype, int64_t ldo, int shares, int64_t
                           int vec, hipStream_t stream) {
   const int k_tiles = static_cast<int>(mx_tiles(K, 128));
   const MxMatrix ma = matrix_of(a, M, K, a_kind), mw = matrix_of(w, N, K, kE2M1);
-  if (form != kMxStream) return launch_mx_tiles(form, out, dtype, ldo, shares, share_stride, ma, a_kind, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec, stream);
-  // (as many tiles of the matrix as of rows: what is read of the rows, and e4m3 taken apart, serves them all)
-  const int mt = stream_tiles(M);
-  const dim3 grid((mw.tiles + mt - 1) / mt, (ma.tiles + mt - 1) / mt, shares);
-#define GO(T, ACT, MT) mx_stream_kernel<T, ACT, MT, MT, (MT == 4 ? 4 : 8)><<<grid, (MT == 4 ? 256 : 512), 0, stream>>>(static_cast<T*>(out), ldo, share_stride, ma, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec)
-#define GO_MT(T, ACT) do { if (mt == 1) GO(T, ACT, 1); else if (mt == 2) GO(T, ACT, 2); else GO(T, ACT, 4); } while (0)
-  if (dtype == kF32) { if (a_kind == kE2M1) GO_MT(float, kE2M1); else GO_MT(float, kE4M3); }
-  else { if (a_kind == kE2M1) GO_MT(bf16_t, kE2M1); else GO_MT(bf16_t, kE4M3); }
-#undef GO_MT
+  if (form != kMxStream && form != kMxStream64x64) return launch_mx_tiles(form, out, dtype, ldo, shares, share_stride, ma, a_kind, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec, stream);
+  const int mt = form == kMxStream64x64 ? 4 : stream_tiles(M, false), nt = form == kMxStream64x64 ? 4 : mt > 1 ? 2 : 1;
+  const dim3 grid((mw.tiles + nt - 1) / nt, (ma.tiles + mt - 1) / mt, shares);
+#define GO(T, ACT, NT, MT, WAVES) mx_stream_kernel<T, ACT, NT, MT, WAVES><<<grid, WAVES * 64, 0, stream>>>(static_cast<T*>(out), ldo, share_stride, ma, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec)
+#define GO_FORM(T, ACT) do { if (nt == 4) GO(T, ACT, 4, 4, 4); else if (mt == 4) GO(T, ACT, 2, 4, 8); else if (mt == 2) GO(T, ACT, 2, 2, 8); else GO(T, ACT, 1, 1, 8); } while (0)
+  if (dtype == kF32) { if (a_kind == kE2M1) GO_FORM(float, kE2M1); else GO_FORM(float, kE4M3); }
+  else { if (a_kind == kE2M1) GO_FORM(bf16_t, kE2M1); else GO_FORM(bf16_t, kE4M3); }
+#undef GO_FORM
 #undef GO
   return check_launch("gemm_mx");
 }
@@ -334,10 +342,11 @@ extern "C" int alofa_gemm_swiglu_mx(void* out, int out_kind, const void* a, int 
   ALOFA_REQUIRE(form >= -1 && form < kMxForms, "gemm_swiglu_mx: form=%d", form);
   if (form < 0) form = plan_for(M, 256 * static_cast<int64_t>(out_tiles), k_tiles, a_kind, true, 1).form;
   if (form != kMxStream) return launch_mx_tiles_gated(form, static_cast<uint8_t*>(out), out_kind, at, out_tiles, ma, a_kind, mg, mu, static_cast<int>(M), static_cast<int>(N), k_tiles, gelu != 0, stream);
-  const int mt = stream_tiles(M);
+  const int mt = stream_tiles(M, true);
+  ALOFA_REQUIRE(mx_tiles(ma.tiles, mt) <= 65535, "gemm_swiglu_mx: more rows than the streaming kernel's grid has room for: %lld", static_cast<long long>(M));
   const dim3 grid(4 * out_tiles, (ma.tiles + mt - 1) / mt);
 #define GO(ACT, OUT, MT) mx_stream_gated_kernel<ACT, OUT, MT, 4><<<grid, 256, 0, stream>>>(static_cast<uint8_t*>(out), at, out_tiles, ma, mg, mu, static_cast<int>(M), static_cast<int>(N), k_tiles, gelu)
-#define GO_MT(ACT, OUT) do { if (mt == 1) GO(ACT, OUT, 1); else if (mt == 2) GO(ACT, OUT, 2); else GO(ACT, OUT, 4); } while (0)
+#define GO_MT(ACT, OUT) do { if (mt == 1) GO(ACT, OUT, 1); else GO(ACT, OUT, 2); } while (0)
   if (a_kind == kE2M1) { if (out_kind == kE2M1) GO_MT(kE2M1, kE2M1); else GO_MT(kE2M1, kE4M3); }
   else { if (out_kind == kE2M1) GO_MT(kE4M3, kE2M1); else GO_MT(kE4M3, kE4M3); }
 #undef GO_MT

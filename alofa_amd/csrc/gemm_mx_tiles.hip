@@ -4,6 +4,11 @@
 // outputs of one row side by side). Slabs of 128 along K come from memory straight into a ring of S slabs in LDS (global_load_lds); elements and scales lie in memory as the
 // fragments are read, so a slab is whole runs of 1 KB, one per wave and instruction, and 16 lanes' fragments are 256 bytes in a row: nothing is permuted and no banks meet.
 //
+// A block of four waves and fewer outputs than a compute unit can work on at once has two teams (KS = 2): each multiplies one half of every slab, 64 along K, and the second's sums go to the first at the end. A wave's own
+// products and arithmetic do not overlap (a turn of 357 cycles of products and one of 121 of arithmetic took 469 together), another wave's do: tiles of 64 x 64 took 13.1 us where one team took 18.9 (64 rows against
+// 4,608 x 3,584), of 128 x 128 25.4 for 27.8 (and 42.5 for 44.0, 333 rows against 18,944 x 3,584).
+// Many rows are bound by the products' rate, at which the card's power allows 4.1 to 4.3 PFLOP/s of e4m3 instructions, i.e. 2.1 of products in two passes, and 5.3 to 6.2 of e2m1: 2,048 x 8,192 x 8,192 runs at 1.6 and 3.9.
+//
 // Operands of the instruction, lane l: row l % 32; e2m1: the 32 numbers from 32 (l / 32) on; e4m3: the sixteen from 16 (l / 32) on and the sixteen from 32 + 16 (l / 32) on; the scale of block
 // l / 32. acc[e] holds the matrix's row 8 (e / 4) + 4 (l / 32) + e % 4 against the activations' row l % 32.
 #include "gemm_mx.h"
@@ -11,15 +16,16 @@
 
 namespace alofa {
 
-template <int kAct, int NF_, int MF_, int WN_, int WM_, int S_>
+template <int kAct, int NF_, int MF_, int WN_, int WM_, int S_, int KS_ = 1>
 struct MxTile {
-  static constexpr int NF = NF_, MF = MF_, WN = WN_, WM = WM_, S = S_, kWaves = WN * WM;
+  static constexpr int NF = NF_, MF = MF_, WN = WN_, WM = WM_, S = S_, KS = KS_, kTeam = WN * WM, kWaves = kTeam * KS;
   static constexpr int BN = 32 * NF * WN, BM = 32 * MF * WM;
   static constexpr int kRowsPieces = BM / 16 * (kAct == kE2M1 ? 1 : 2), kPieces = BN / 16 + kRowsPieces;      // of 1 KB
   static_assert((BN + BM) / 64 <= kWaves, "a wave brings the scales of four tiles at most");
   static constexpr int kLoads = (kPieces + kWaves - 1) / kWaves + 1;    // a wave's, per slab (a wave with a piece less brings its first one again)
   static constexpr int kScales = kPieces * 1024, kSlab = kScales + kWaves * 256;
   static_assert(S >= 2 && S * kSlab <= 160 * 1024 && (S - 2) * kLoads < 64, "the ring fits LDS, what is on its way is counted");
+  static_assert(KS == 1 || (KS == 2 && kTeam * NF * MF * 4096 <= S * kSlab), "a slab has two halves of 64; their sums meet in the ring");
 };
 
 // A wave's loads of a slab have come, and its reads from LDS; those of `behind` slabs behind it, kMost at most, stay on their way.
@@ -34,7 +40,7 @@ template <int kAct, typename T, bool kGated>
 __device__ __forceinline__ void mx_tile_product(char* ring, const MxMatrix a, const MxMatrix w, const MxMatrix w2, int m_tile, int n_tile, int k_begin, int k_end, int k_tiles, f32x16 (&acc)[T::NF][T::MF]) {
   constexpr int NF = T::NF, MF = T::MF, S = T::S, kLoads = T::kLoads, kMatrixPieces = T::BN / 16, kHalf = kMatrixPieces / 2;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-  const int wn = wave % T::WN, wm = wave / T::WN;
+  const int wn = wave % T::WN, wm = wave % T::kTeam / T::WN, team = wave / T::kTeam;
 
   // what this wave brings: pieces wave, wave + kWaves, ..; a piece is a run of 1 KB (tiles behind the last of a matrix come from the last; their results are not stored)
   const uint8_t *const units = w.units, *const up_units = w2.units, *const scales_of = w.scales, *const up_scales = w2.scales;
@@ -97,7 +103,7 @@ __device__ __forceinline__ void mx_tile_product(char* ring, const MxMatrix a, co
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
   // where this lane's fragments lie within a slab
-  const int half = lane / 32, shift = 8 * half, in_tile = lane % 16 * 16;
+  const int half = lane / 32, shift = 8 * half + 16 * team, in_tile = lane % 16 * 16;
   int w_tile[NF], a_tile[MF];
 #pragma unroll
   for (int i = 0; i < NF; ++i) w_tile[i] = kGated ? (i < NF / 2 ? (wn * (NF / 2) + i) * 2 : kHalf + (wn * (NF / 2) + i - NF / 2) * 2) : (wn * NF + i) * 2;
@@ -117,17 +123,17 @@ __device__ __forceinline__ void mx_tile_product(char* ring, const MxMatrix a, co
       i32x8 wf[NF], af[MF][kAct == kE2M1 ? 1 : 2];
 #pragma unroll
       for (int i = 0; i < NF; ++i) {
-        const uint4 v = *reinterpret_cast<const uint4*>(slab + (w_tile[i] + odd) * 1024 + (2 * s + half) * 256 + in_tile);
+        const uint4 v = *reinterpret_cast<const uint4*>(slab + (w_tile[i] + odd) * 1024 + (2 * (s + team) + half) * 256 + in_tile);
         wf[i] = {static_cast<int>(v.x), static_cast<int>(v.y), static_cast<int>(v.z), static_cast<int>(v.w), 0, 0, 0, 0};
       }
 #pragma unroll
       for (int j = 0; j < MF; ++j) {
         const char* rows = slab + kMatrixPieces * 1024;
         if constexpr (kAct == kE2M1) {
-          const uint4 v = *reinterpret_cast<const uint4*>(rows + (a_tile[j] + odd) * 1024 + (2 * s + half) * 256 + in_tile);
+          const uint4 v = *reinterpret_cast<const uint4*>(rows + (a_tile[j] + odd) * 1024 + (2 * (s + team) + half) * 256 + in_tile);
           af[j][0] = {static_cast<int>(v.x), static_cast<int>(v.y), static_cast<int>(v.z), static_cast<int>(v.w), 0, 0, 0, 0};
         } else {
-          const char* at = rows + (a_tile[j] + odd) * 2048 + (4 * s + half) * 256 + in_tile;
+          const char* at = rows + (a_tile[j] + odd) * 2048 + (4 * (s + team) + half) * 256 + in_tile;
           const uint4 lo = *reinterpret_cast<const uint4*>(at), hi = *reinterpret_cast<const uint4*>(at + 512);
           const uint32_t x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
@@ -146,7 +152,7 @@ __device__ __forceinline__ void mx_tile_product(char* ring, const MxMatrix a, co
           for (int i = 0; i < NF; ++i) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf[i], af[j][part], acc[i][j], kE2M1, kAct, 2 * s, ws[i], 2 * s, as[j]);
     };
     step64(std::integral_constant<int, 0>{});
-    step64(std::integral_constant<int, 1>{});
+    if constexpr (T::KS == 1) step64(std::integral_constant<int, 1>{});
   };
 
   // Slab k + S - 1 is set out once every wave has read slab k - 1, whose place it takes, i.e. behind the barrier of step k. A wave waits for its own loads of slab k (those of the S - 2 behind it
@@ -171,6 +177,30 @@ __device__ __forceinline__ void mx_tile_product(char* ring, const MxMatrix a, co
     }
     multiply(ring + at);
     at = advance(at);
+  }
+  if constexpr (T::KS == 2) {      // the second team's sums, to the first
+    __syncthreads();
+    float4* sums = reinterpret_cast<float4*>(ring) + wave % T::kTeam * (NF * MF * 256) + lane;
+    if (team == 1) {
+#pragma unroll
+      for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int j = 0; j < MF; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) sums[((i * MF + j) * 4 + q) * 64] = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+    }
+    __syncthreads();
+    if (team == 0) {
+#pragma unroll
+      for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int j = 0; j < MF; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4 v = sums[((i * MF + j) * 4 + q) * 64];
+            acc[i][j][4 * q] += v.x, acc[i][j][4 * q + 1] += v.y, acc[i][j][4 * q + 2] += v.z, acc[i][j][4 * q + 3] += v.w;
+          }
+    }
   }
 }
 
@@ -248,7 +278,8 @@ __global__ void __launch_bounds__(T::kWaves * 64) mx_tile_kernel(TO* __restrict_
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, wn = wave % T::WN, wm = wave / T::WN;
   out += place.share * share_stride;
   __syncthreads();      // (the ring is free: nothing is on its way, and every wave has read the last slab)
-  static_assert(T::kWaves * kRoom<TO> <= sizeof(ring), "the rows' way out fits the ring");
+  if (wave >= T::kTeam) return;
+  static_assert(T::kTeam * kRoom<TO> <= sizeof(ring), "the rows' way out fits the ring");
   char* room = ring + wave * kRoom<TO>;
 #pragma unroll
   for (int j = 0; j < T::MF; ++j) {
@@ -281,6 +312,7 @@ __global__ void __launch_bounds__(T::kWaves * 64) mx_tile_gated_kernel(uint8_t* 
   f32x16 acc[T::NF][T::MF];
   mx_tile_product<kAct, T, true>(ring, a, gate, up, place.bm * (T::BM / 16), place.bn * (T::BN / 32), 0, k_tiles, k_tiles, acc);
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, wn = wave % T::WN, wm = wave / T::WN, half = lane / 32;
+  if (wave >= T::kTeam) return;
 #pragma unroll
   for (int j = 0; j < T::MF; ++j)
 #pragma unroll
@@ -342,10 +374,10 @@ template <int kAct> using T256x256 = MxTile<kAct, kAct == kE2M1 ? 4 : 8, kAct ==
 template <int kAct> using T256x192 = MxTile<kAct, 6, 1, 1, 8, 3>;
 template <int kAct> using T256x160 = MxTile<kAct, 5, 1, 1, 8, 3>;
 template <int kAct> using T256x128 = MxTile<kAct, 4, 1, 1, 8, 3>;
-template <int kAct> using T128x128 = MxTile<kAct, 4, 1, 1, 4, 3>;
-template <int kAct> using T128x64 = MxTile<kAct, 2, 1, 1, 4, 3>;
-template <int kAct> using T64x128 = MxTile<kAct, 2, 1, 2, 2, 4>;
-template <int kAct> using T64x64 = MxTile<kAct, 2, 1, 1, 2, 4>;
+template <int kAct> using T128x128 = MxTile<kAct, 4, 1, 1, 4, kAct == kE2M1 ? 4 : 3, 2>;
+template <int kAct> using T128x64 = MxTile<kAct, 2, 1, 1, 4, 3, 2>;
+template <int kAct> using T64x128 = MxTile<kAct, 2, 1, 2, 2, 4, 2>;
+template <int kAct> using T64x64 = MxTile<kAct, 2, 1, 1, 2, 4, 2>;
 
 }  // namespace
 
