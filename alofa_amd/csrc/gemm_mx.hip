@@ -241,7 +241,7 @@ constexpr MxCost kMxStream8[] = {{kMxStream, 16, 16, 8, 0.4f, 0.4f, 4.3f, 0.f}, 
 constexpr MxCost kMxStream4[] = {{kMxStream, 16, 16, 8, 0.25f, 0.25f, 4.3f, 0.f}, {kMxStream, 32, 32, 8, 0.45f, 0.45f, 4.3f, 0.f}, {kMxStream, 64, 32, 8, 0.47f, 0.47f, 4.3f, 0.5f},
                                  {kMxStream, 16, 64, 4, 0.55f, 0.55f, 4.3f, 0.f}, {kMxStream, 32, 64, 4, 0.55f, 0.55f, 4.3f, 0.f}};
 constexpr MxCost kMxWide8 = {kMxStream64x64, 64, 64, 4, 0.87f, 0.77f, 4.3f, 1.1f}, kMxWide4 = {kMxStream64x64, 64, 64, 4, 0.45f, 0.36f, 4.3f, 1.5f};
-constexpr int kMxStreamRows = 512;      // most rows that the streaming kernel is asked for (the largest products measured with it)
+constexpr int kMxStreamRows = 2048;      // most rows that the streaming kernel is asked for (measured up to 1,500: what it reads again and again costs more than a slab in LDS but where the matrix is small)
 
 struct MxPlan {
   int form, shares;
