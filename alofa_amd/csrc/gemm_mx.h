@@ -57,7 +57,7 @@ __device__ __forceinline__ void mx_store4(TO* __restrict__ out, int64_t ldo, con
     if (n + e < N) store_f32(to + e, epilogue == kMxResidual ? load_f32(to + e) + v[e] : v[e]);
 }
 
-// Which kernel: the one that streams the matrix (gemm_mx.hip), or tiles of so many rows by so many columns (gemm_mx_tiles.hip; with a gate: columns of gate and up together)
+// Which kernel: the one that streams the matrix (gemm_mx.hip), by as many tiles of 16 as there are rows for or by four and four, or tiles of so many rows by so many columns (gemm_mx_tiles.hip; with a gate: columns of gate and up together)
 enum MxForm : int { kMxStream = 0, kMx256x256 = 1, kMx256x192 = 2, kMx256x160 = 3, kMx256x128 = 4, kMx128x128 = 5, kMx128x64 = 6, kMx64x64 = 7, kMx64x128 = 8, kMxStream64x64 = 9, kMxForms = 10 };
 
 int launch_mx_tiles(int form, void* out, int dtype, int64_t ldo, int shares, int64_t share_stride, const MxMatrix& a, int a_kind, const MxMatrix& w, const float* bias, int M, int N, int k_tiles, int epilogue, bool vec,

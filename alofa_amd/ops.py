@@ -2966,7 +2966,7 @@ def rmsnorm_mx(out: MXRows, x: torch.Tensor, w: torch.Tensor, eps: float, add: O
     _call("alofa_rmsnorm_mx", out.buffer, kind, x, ldx, add, shares, stride, ld_add, total, ld_total, w, _F(eps), out.rows, out.k, _stream())
 
 
-MX_FORMS = {None: -1, "stream": 0, "256x256": 1, "256x192": 2, "256x160": 3, "256x128": 4, "128x128": 5, "128x64": 6, "64x64": 7, "64x128": 8, "stream64x64": 9}      # (as csrc/gemm_mx.h numbers them: the streaming kernel, or tiles of rows x columns)
+MX_FORMS = {None: -1, "stream": 0, "256x256": 1, "256x192": 2, "256x160": 3, "256x128": 4, "128x128": 5, "128x64": 6, "64x64": 7, "64x128": 8, "stream64x64": 9}      # (as csrc/gemm_mx.h numbers them: the streaming kernel with the tiles that its rows ask for or four by four, or tiles of rows x columns in LDS)
 
 
 def _mx_form(kernel: Optional[str]) -> int:
