@@ -3041,7 +3041,8 @@ def gemm_mx_shares(out: torch.Tensor, a: MXRows, w: MXRows, kernel: Optional[str
 
 
 def gemm_swiglu_mx(out: MXRows, a: MXRows, w_gate: MXRows, w_up: MXRows, act: str = "silu", kernel: Optional[str] = None) -> None:
-    """out [M, N] = act(a @ w_gate.T) * (a @ w_up.T) as microscaled rows, act "silu" or "gelu_tanh"; the products and the gate in float32. ``kernel`` as for ``gemm_mx``."""
+    """out [M, N] = act(a @ w_gate.T) * (a @ w_up.T) as microscaled rows, act "silu" or "gelu_tanh"; the products and the gate in float32. ``kernel`` as for ``gemm_mx``, but
+    for "256x160" and "stream64x64", which this product does not have."""
     if act not in GATED:
         raise AlofaError("unsupported", "no such activation of a gate", f"act={act}")
     kind, M, N, K = _mx_product(a, w_gate, "w_gate")

@@ -517,3 +517,13 @@ def test_more_rows_than_a_norms_launch_takes_are_refused():
         ops.rmsnorm_mx(out, torch.ones(1, 32, device=DEV).expand(rows, 32), torch.ones(32, device=DEV), 1e-6)
     torch.cuda.synchronize()
     assert not out.buffer[:64].any()
+
+
+@pytest.mark.parametrize("kernel", ["256x160", "stream64x64"])
+def test_forms_that_gated_products_do_not_have_are_refused(kernel):
+    a, w, out = made(numbers(40, 64, 1), "e4m3"), made(numbers(32, 64, 2), "e2m1"), ops.MXRows(40, 32, "e4m3", DEV)
+    out.buffer.fill_(7)
+    with pytest.raises(AlofaError):
+        ops.gemm_swiglu_mx(out, a, w, w, kernel=kernel)
+    torch.cuda.synchronize()
+    assert (out.buffer == 7).all()
