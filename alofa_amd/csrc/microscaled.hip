@@ -168,13 +168,14 @@ __device__ __forceinline__ void add_shares(const float* __restrict__ row, int64_
 
 // total = x + (add[0] + add[1] + ..) in float, y = total / sqrt(mean(total^2) + eps) * w in double, y to microscaled rows. A block takes a row. The squares' sum and
 // y are in double so that no element depends on the order of a sum: a value next to the middle of two elements would become one or the other.
-// Memory bounds many rows: 2,048 x 3,584 with one share 27.2 us (3.5 TB/s), 2,048 x 5,120 with two 46 (3.9); few are bound by one row's steps one after the other, 4.3 us at 1 x 896 and 6.5 at 64 x 5,120 with four
-// shares. A block of four rows would write 64 bytes at a time for 16: 26.1 us at 2,048 rows, but 11.6 for 7.8 at 512.
-// kGroups > 0: a row of at most 2,048 kGroups numbers stays in registers between the sum and the scaling; 0: any row, read twice.
-template <int kKind, int kGroups, bool kVec>
-__global__ void __launch_bounds__(256) rmsnorm_mx_kernel(uint8_t* __restrict__ out, int64_t scales_at, const float* x, int64_t ldx, const float* __restrict__ add, int shares,
+// Memory bounds many rows: 2,048 x 3,584 with one share 26.8 us (3.6 TB/s), 2,048 x 5,120 with two 44.8 (4.0); few are bound by one row's steps one after the other, 4.3 us at 1 x 896 and 5.4 at 64 x 5,120 with four
+// shares. A block of four rows would write 64 bytes at a time for 16: 26.1 us at 2,048 rows, but 11.6 for 8.0 at 512.
+// kStay: a row of at most 8 kThreads numbers (8,192) stays in registers between the sum and the scaling, eight a thread; else any row, read twice. (256 threads with two and three eights took 6.5 us for 5.4 at
+// 64 x 5,120 and 27.2 for 26.8 at 2,048 x 3,584: a row's steps are shorter.)
+template <int kKind, int kThreads, bool kStay, bool kVec>
+__global__ void __launch_bounds__(kThreads) rmsnorm_mx_kernel(uint8_t* __restrict__ out, int64_t scales_at, const float* x, int64_t ldx, const float* __restrict__ add, int shares,
                                                          int64_t share_stride, int64_t ld_add, float* total, int64_t ld_total, const float* __restrict__ w, float eps, int k, int k_tiles) {
-  __shared__ double scratch[4];
+  __shared__ double scratch[kThreads / kWave];
   const int64_t r = blockIdx.x;
   const int per_row = 16 * k_tiles;
   auto take = [&](int c, float (&v)[8]) {
@@ -204,35 +205,27 @@ __global__ void __launch_bounds__(256) rmsnorm_mx_kernel(uint8_t* __restrict__ o
     put8<kKind>(out, scales_at, r, c, k_tiles, v);
   };
   double ss = 0;
-  if constexpr (kGroups > 0) {
-    float v[kGroups][8], weight[kGroups][8];
+  if constexpr (kStay) {
+    const int c = threadIdx.x;
+    float v[8], weight[8];
+    load8<float, kVec>(w, 8 * c, k, weight);
+    take(c, v);      // (nothing but zeros behind the row's end)
+    keep(c, v);
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) load8<float, kVec>(w, 8 * (static_cast<int>(threadIdx.x) + 256 * i), k, weight[i]);
-#pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
-      const int c = threadIdx.x + 256 * i;
-      take(c, v[i]);      // (nothing but zeros behind the row's end)
-      keep(c, v[i]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss += static_cast<double>(v[i][e]) * static_cast<double>(v[i][e]);
-    }
-    ss = block_sum<double, 256>(ss, scratch);
+    for (int e = 0; e < 8; ++e) ss += static_cast<double>(v[e]) * static_cast<double>(v[e]);
+    ss = block_sum<double, kThreads>(ss, scratch);
     const double scale = 1.0 / sqrt(ss / static_cast<double>(k) + static_cast<double>(eps));
-#pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
-      const int c = threadIdx.x + 256 * i;
-      if (c < per_row) leave(c, v[i], weight[i], scale);
-    }
+    if (c < per_row) leave(c, v, weight, scale);
   } else {
-    for (int c = threadIdx.x; c < per_row; c += 256) {
+    for (int c = threadIdx.x; c < per_row; c += kThreads) {
       float v[8];
       take(c, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss += static_cast<double>(v[e]) * static_cast<double>(v[e]);
     }
-    ss = block_sum<double, 256>(ss, scratch);
+    ss = block_sum<double, kThreads>(ss, scratch);
     const double scale = 1.0 / sqrt(ss / static_cast<double>(k) + static_cast<double>(eps));
-    for (int c = threadIdx.x; c < per_row; c += 256) {
+    for (int c = threadIdx.x; c < per_row; c += kThreads) {
       float v[8];
       take(c, v);      // (`total` may be x itself: a thread reads its numbers again before it writes them)
       keep(c, v);
@@ -314,12 +307,12 @@ extern "C" int alofa_rmsnorm_mx(void* out, int kind, const float* x, int64_t ldx
   const int k_tiles = static_cast<int>(mx_tiles(k, 128)), n = static_cast<int>(k);
   const int64_t at = mx_scales_at(rows, k, kind);
   const bool vec = k % 8 == 0 && aligned16(x) && ldx % 4 == 0 && aligned16(w) && (shares == 0 || (aligned16(add) && ld_add % 4 == 0 && share_stride % 4 == 0)) && (!total || (aligned16(total) && ld_total % 4 == 0));
-  const int groups = (16 * k_tiles + 255) / 256;
-#define GO(KIND, G, VEC) rmsnorm_mx_kernel<KIND, G, VEC><<<static_cast<unsigned>(rows), 256, 0, stream>>>(static_cast<uint8_t*>(out), at, x, ldx, add, shares, share_stride, ld_add, total, ld_total, w, eps, n, k_tiles)
-#define GO_VEC(KIND, G) do { if (vec) GO(KIND, G, true); else GO(KIND, G, false); } while (0)
-#define GO_GROUPS(KIND) do { if (groups == 1) GO_VEC(KIND, 1); else if (groups == 2) GO_VEC(KIND, 2); else if (groups == 3) GO_VEC(KIND, 3); else if (groups == 4) GO_VEC(KIND, 4); else GO_VEC(KIND, 0); } while (0)
-  if (kind == kE2M1) GO_GROUPS(kE2M1); else GO_GROUPS(kE4M3);
-#undef GO_GROUPS
+  const int units = 16 * k_tiles;
+#define GO(KIND, THREADS, STAY, VEC) rmsnorm_mx_kernel<KIND, THREADS, STAY, VEC><<<static_cast<unsigned>(rows), THREADS, 0, stream>>>(static_cast<uint8_t*>(out), at, x, ldx, add, shares, share_stride, ld_add, total, ld_total, w, eps, n, k_tiles)
+#define GO_VEC(KIND, THREADS, STAY) do { if (vec) GO(KIND, THREADS, STAY, true); else GO(KIND, THREADS, STAY, false); } while (0)
+#define GO_WIDTH(KIND) do { if (units <= 256) GO_VEC(KIND, 256, true); else if (units <= 512) GO_VEC(KIND, 512, true); else if (units <= 768) GO_VEC(KIND, 768, true); else if (units <= 1024) GO_VEC(KIND, 1024, true); else GO_VEC(KIND, 256, false); } while (0)
+  if (kind == kE2M1) GO_WIDTH(kE2M1); else GO_WIDTH(kE4M3);
+#undef GO_WIDTH
 #undef GO_VEC
 #undef GO
   return check_launch("rmsnorm_mx");
