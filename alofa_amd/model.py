@@ -172,7 +172,7 @@ class Model:
             nxt = self.blocks[self.order[i + 1].layer] if i + 1 < len(self.order) and self.order[i + 1].join is None else None
             norm = nxt.wants_normed(rows) if nxt is not None and nxt.takes_normed else None
             leaves = norm is not None and block.can_leave(norm)
-            then = (norm, ctx.scratch("normed", tuple(hidden.shape), self.rt.dtype)) if leaves else None
+            then = (norm, nxt.normed_rows(ctx, hidden)) if leaves else None
             if self.streams and nxt is None:
                 then = (self.sum_of_streams, hidden)
             if tapes is not None and i in tapes.sources:

@@ -281,6 +281,10 @@ class Block(Part):
     def wants_normed(self, rows: int):
         return None
 
+    def normed_rows(self, ctx, hidden):
+        """Where the rows that it is handed as ``normed`` are left."""
+        return ctx.scratch("normed", tuple(hidden.shape), self.rt.dtype)
+
     def can_leave(self, norm) -> bool:
         """Whether this block's last launch can leave what the next block asks for (its ``wants_normed``)."""
         return norm.as_rmsnorm() is not None

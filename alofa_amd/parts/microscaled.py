@@ -5,7 +5,8 @@ it was: the stream and all sums in float32, queries, keys and values in bfloat16
 
 a = stream; n0 = q8(norm0(a)); qkv = n0 Wqkv^T + b; o = q8(attention(qkv)); a += o Wo^T; n1 = q8(norm1(a)); a += q8(act(n1 Wg^T) * (n1 Wu^T)) Wd^T
 
-The output product leaves the shares of its sum and the norm behind it adds them to the stream on its way."""
+The output product leaves the shares of its sum and the norm behind it adds them to the stream on its way. So does the product down, where its sum is
+shared out, with the first norm of the next such layer (a launch less: 4.6 us of 106 a layer, 64 rows at 3,584 x 18,944)."""
 from __future__ import annotations
 
 import dataclasses
@@ -33,8 +34,25 @@ def microscaled(spec: ModelSpec) -> ModelSpec:
     return dataclasses.replace(spec, layers=type(spec.layers)(layers))
 
 
+class _MicroscaledNorm:
+    """The norm that a layer starts with, as what it asks the layer before for: rows that no other block leaves."""
+
+    def __init__(self, norm):
+        self.norm = norm
+
+    def as_rmsnorm(self):
+        return None
+
+
 class MicroscaledPreNorm(PreNormBlock):
-    takes_normed = False      # (its norms leave microscaled rows, which no other part gives)
+    def wants_normed(self, rows):
+        return _MicroscaledNorm(self.norms[0])
+
+    def can_leave(self, norm):
+        return isinstance(norm, _MicroscaledNorm)
+
+    def normed_rows(self, ctx, hidden):
+        return self._rows(ctx, "mx_normed", *hidden.shape)
 
     def __init__(self, layer, weights, rt):
         if rt.exact:
@@ -55,10 +73,11 @@ class MicroscaledPreNorm(PreNormBlock):
     def _rows(ctx, name: str, rows: int, k: int) -> ops.MXRows:
         return ops.MXRows(rows, k, "e4m3", buffer=ctx.scratch(name, (ops.MXRows.bytes(rows, k, "e4m3"),), torch.uint8))
 
-    def forward(self, ctx, entry, hidden):
+    def forward(self, ctx, entry, hidden, normed=None, then=None):
         (T, h), m, f = hidden.shape, self.mixer, self.feed_forward
-        normed = self._rows(ctx, "mx_normed", T, h)
-        ops.rmsnorm_mx(normed, hidden, *self.norms[0].as_rmsnorm())
+        if normed is None:
+            normed = self.normed_rows(ctx, hidden)
+            ops.rmsnorm_mx(normed, hidden, *self.norms[0].as_rmsnorm())
         qkv = ctx.scratch("qkv", (T, m.qkv_width), self.rt.dtype)
         ops.gemm_mx(qkv, normed, self.w_qkv, m.b_qkv, scratch=ctx.scratch)
         attn = ctx.scratch("attn", (T, m.heads * m.d), self.rt.dtype)
@@ -74,7 +93,15 @@ class MicroscaledPreNorm(PreNormBlock):
         ops.rmsnorm_mx(normed, hidden, *self.norms[1].as_rmsnorm(), add=mixed, total=hidden)
         act = self._rows(ctx, "mx_act", T, f.intermediate)
         ops.gemm_swiglu_mx(act, normed, self.w_gate, self.w_up, f.activation)
-        ops.gemm_mx(hidden, act, self.w_down, add_to_out=True, scratch=ctx.scratch)
+        shares = 1 if then is None else ops.mx_shares(T, h, f.intermediate)
+        if shares == 1:      # (whole sums are added where they are formed: a norm that adds them would read and write the stream once more)
+            ops.gemm_mx(hidden, act, self.w_down, add_to_out=True, scratch=ctx.scratch)
+            return False
+        down = ctx.scratch("mx_down", (shares, T, h), torch.float32)
+        ops.gemm_mx_shares(down, act, self.w_down)
+        norm, rows = then
+        ops.rmsnorm_mx(rows, hidden, *norm.norm.as_rmsnorm(), add=down, total=hidden)
+        return True
 
 
 register_part("block", KIND, MicroscaledPreNorm)

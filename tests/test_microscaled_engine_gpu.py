@@ -132,3 +132,19 @@ def test_programs(tiny_dirs, tmp_path):
                        input=step + "\n", capture_output=True, text=True, timeout=110)
     assert r.returncode == 0, r.stderr
     assert int(np.fromfile(tmp_path / "0.f32", dtype=np.float32).argmax()) == want[0][0]
+
+
+def test_shares_of_the_product_down_go_to_the_next_layers_norm(tmp_path):
+    """A feed-forward so wide that its sum is shared out over K: the next layer's first norm adds the shares to the stream."""
+    from alofa_amd import ops
+    from alofa_amd.replay import Replayer
+    from alofa_amd.weights import write_random_model
+    cfg = dict(TINY["A"], num_hidden_layers=3, intermediate_size=8192)
+    write_random_model(cfg, tmp_path, seed=77)
+    ids = random_ids(5, 90, cfg["vocab_size"])
+    replayer = Replayer(tmp_path, "bfloat16", 256, matrices="mxfp4")
+    assert all(ops.mx_shares(n, cfg["hidden_size"], 8192) > 1 for n in (1, 17, 40, 90))
+    ref = reference(tmp_path, ids)
+    assert_close(collect(replayer, whole("w", ids))["w"], ref, "bfloat16", "whole")
+    assert_close(collect(replayer, portions("p", ids, (40, 17, 23, 10)))["p"], ref, "bfloat16", "portions")
+    assert_close(collect(replayer, bulk_and_tail("b", ids, 84))["b"], ref, "bfloat16", "bulk then one by one")
