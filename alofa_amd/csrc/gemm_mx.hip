@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(256) mx_sum_kernel(TO* __restrict__ out, int64
 }
 
 // What a product takes in each form, in us, and how it is chosen: besides + more (each - 1) + turns max(alone, each * of_each), where a compute unit has `each` blocks and a block takes `step` slabs of 128 along K in a
-// turn. Fitted to 1,200 measured products (1 to 2,048 rows, matrices of 1,152 x 896 to 18,944 x 3,584 and 3,584 x 18,944; 3 % off in the mean with e4m3, 6 % with e2m1). Read along a column: tiles of 256 x 256 pay where all
+// turn. Fitted to 2,400 measured products (1 to 2,048 rows, matrices of 1,152 x 896 to 18,944 x 3,584 and 3,584 x 18,944; 3 % off in the mean with e4m3, 6 % with e2m1). Read along a column: tiles of 256 x 256 pay where all
 // compute units have some, small ones and the streaming kernel where blocks are few: 333 rows against 4,608 x 3,584 take 15.5 us by 64 x 64 streamed, 16.8 and 17.8 by tiles of 64 x 64 and 64 x 128, 25.4 by 128 x 128 and 41 by
 // 256 x 128; 700 rows against 18,944 x 3,584 91, 94, 80 and 85. A sum that is shared out over K takes a launch more, which adds the shares up, unless a norm does.
 struct MxCost {

@@ -527,3 +527,16 @@ def test_forms_that_gated_products_do_not_have_are_refused(kernel):
         ops.gemm_swiglu_mx(out, a, w, w, kernel=kernel)
     torch.cuda.synchronize()
     assert (out.buffer == 7).all()
+
+
+@pytest.mark.parametrize("kernel", FORMS)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("M,N,K,shares", [(3, 40, 260, 3), (70, 290, 1100, 4), (300, 136, 900, 8)])
+def test_every_kernel_takes_shares(M, N, K, shares, kind, kernel):
+    a, w, av, wv = operands(M, N, K, kind, M + K)
+    parts = torch.full((shares, M, N), float("nan"), device=DEV)
+    ops.gemm_mx_shares(parts, a, w, kernel=kernel)
+    tiles, got = -(-K // 128), parts.double().cpu().numpy()
+    for s in range(shares):
+        cut = slice(128 * (tiles * s // shares), 128 * (tiles * (s + 1) // shares))
+        assert (np.abs(got[s] - av[:, cut] @ wv[:, cut].T) <= off_by(av[:, cut], wv[:, cut])).all()
