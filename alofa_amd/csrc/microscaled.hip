@@ -303,14 +303,14 @@ extern "C" int alofa_rmsnorm_mx(void* out, int kind, const float* x, int64_t ldx
   if (!sizes_fit("rmsnorm_mx", kind, rows, k)) return 1;
   ALOFA_REQUIRE(out && x && w && aligned16(out) && shares >= 0 && (shares == 0 || add) && (shares == 0 || total) && ldx >= 0 && ld_add >= 0 && share_stride >= 0 && ld_total >= 0 && eps > 0.f,
                 "rmsnorm_mx: operands do not fit: shares=%d eps=%g", shares, static_cast<double>(eps));
-  ALOFA_REQUIRE(rows < 1 << 24, "rmsnorm_mx: more rows than a launch takes: %lld", static_cast<long long>(rows));
-  const int k_tiles = static_cast<int>(mx_tiles(k, 128)), n = static_cast<int>(k);
+  const int k_tiles = static_cast<int>(mx_tiles(k, 128)), n = static_cast<int>(k), units = 16 * k_tiles;
+  const int threads = units <= 256 ? 256 : units <= 512 ? 512 : units <= 768 ? 768 : units <= 1024 ? 1024 : 256;
+  ALOFA_REQUIRE(rows * threads < INT64_C(1) << 32, "rmsnorm_mx: more rows than a launch takes: %lld of %lld numbers", static_cast<long long>(rows), static_cast<long long>(k));
   const int64_t at = mx_scales_at(rows, k, kind);
   const bool vec = k % 8 == 0 && aligned16(x) && ldx % 4 == 0 && aligned16(w) && (shares == 0 || (aligned16(add) && ld_add % 4 == 0 && share_stride % 4 == 0)) && (!total || (aligned16(total) && ld_total % 4 == 0));
-  const int units = 16 * k_tiles;
 #define GO(KIND, THREADS, STAY, VEC) rmsnorm_mx_kernel<KIND, THREADS, STAY, VEC><<<static_cast<unsigned>(rows), THREADS, 0, stream>>>(static_cast<uint8_t*>(out), at, x, ldx, add, shares, share_stride, ld_add, total, ld_total, w, eps, n, k_tiles)
 #define GO_VEC(KIND, THREADS, STAY) do { if (vec) GO(KIND, THREADS, STAY, true); else GO(KIND, THREADS, STAY, false); } while (0)
-#define GO_WIDTH(KIND) do { if (units <= 256) GO_VEC(KIND, 256, true); else if (units <= 512) GO_VEC(KIND, 512, true); else if (units <= 768) GO_VEC(KIND, 768, true); else if (units <= 1024) GO_VEC(KIND, 1024, true); else GO_VEC(KIND, 256, false); } while (0)
+#define GO_WIDTH(KIND) do { if (units > 1024) GO_VEC(KIND, 256, false); else if (threads == 256) GO_VEC(KIND, 256, true); else if (threads == 512) GO_VEC(KIND, 512, true); else if (threads == 768) GO_VEC(KIND, 768, true); else GO_VEC(KIND, 1024, true); } while (0)
   if (kind == kE2M1) GO_WIDTH(kE2M1); else GO_WIDTH(kE4M3);
 #undef GO_WIDTH
 #undef GO_VEC

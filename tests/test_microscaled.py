@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from alofa_amd import ops
+from alofa_amd.csrc.build import load
 from alofa_amd.errors import AlofaError
 from plain import microscaled as pm
 
@@ -104,3 +105,26 @@ def test_an_engine_over_a_given_model_does_not_change_its_matrices():
 def test_shares_of_sizes_and_kinds_that_are_refused(M, N, K, kind):
     with pytest.raises(AlofaError):
         ops.mx_shares(M, N, K, kind)
+
+
+# ------------------------------------------------------------- what the entries themselves refuse (addresses of nothing: what is not refused asks for a GPU and finds none)
+
+no_gpu = pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are made up: only for machines on which nothing can be launched")
+A, B, C, D = (1 << (44 + i) for i in range(4))      # apart, and aligned
+
+
+def said(entry, *args):
+    """What the entry refuses its arguments with."""
+    assert ops._answer(entry, *args) != 0
+    return load().alofa_last_error().decode()
+
+
+@no_gpu
+@pytest.mark.parametrize("kind", [0, 4])
+@pytest.mark.parametrize("k,threads", [(32, 256), (2048, 256), (2049, 512), (2176, 512), (4096, 512), (4097, 768), (6144, 768), (6145, 1024), (6272, 1024)])
+def test_a_norms_launch_has_fewer_than_2_32_threads(k, threads, kind):
+    most = ((1 << 32) - 1) // threads
+
+    def norm(rows):
+        return said("alofa_rmsnorm_mx", A, kind, B, 0, None, 0, 0, 0, None, 0, C, 1e-6, rows, k, 0)
+    assert "than a launch takes" in norm(most + 1) and "no ROCm-capable device" in norm(most)
