@@ -291,6 +291,7 @@ static int product_shares(void* out, int dtype, int64_t ldo, int shares, int64_t
   const MxMatrix ma = matrix_of(a, M, K, a_kind), mw = matrix_of(w, N, K, kE2M1);
   if (form != kMxStream && form != kMxStream64x64) return launch_mx_tiles(form, out, dtype, ldo, shares, share_stride, ma, a_kind, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec, stream);
   const int mt = form == kMxStream64x64 ? 4 : stream_tiles(M, false), nt = form == kMxStream64x64 ? 4 : mt > 1 ? 2 : 1;
+  ALOFA_REQUIRE(shares <= 65535, "gemm_mx: more shares than the streaming kernel's grid has room for: %d", shares);
   const dim3 grid((mw.tiles + nt - 1) / nt, (ma.tiles + mt - 1) / mt, shares);
 #define GO(T, ACT, NT, MT, WAVES) mx_stream_kernel<T, ACT, NT, MT, WAVES><<<grid, WAVES * 64, 0, stream>>>(static_cast<T*>(out), ldo, share_stride, ma, mw, bias, static_cast<int>(M), static_cast<int>(N), k_tiles, epilogue, vec)
 #define GO_FORM(T, ACT) do { if (nt == 4) GO(T, ACT, 4, 4, 4); else if (mt == 4) GO(T, ACT, 2, 4, 8); else if (mt == 2) GO(T, ACT, 2, 2, 8); else GO(T, ACT, 1, 1, 8); } while (0)

@@ -3029,7 +3029,8 @@ def mx_shares(M: int, N: int, K: int, kind: str = "e4m3") -> int:
 
 
 def gemm_mx_shares(out: torch.Tensor, a: MXRows, w: MXRows, kernel: Optional[str] = None) -> None:
-    """out [shares, M, N] float32, contiguous: the product a @ w.T, each share the sum over a part of K; ``rmsnorm_mx(add=out)`` adds them up. At most K / 128 shares, rounded up."""
+    """out [shares, M, N] float32, contiguous: the product a @ w.T, each share the sum over a part of K; ``rmsnorm_mx(add=out)`` adds them up. At most K / 128 shares, rounded up, and
+    65,535 by the streaming kernel."""
     kind, M, N, K = _mx_product(a, w)
     _contig("out", _gpu("out", out, torch.float32, 3))
     if tuple(out.shape[1:]) != (M, N) or not 1 <= out.shape[0] <= (K + 127) // 128:

@@ -128,3 +128,14 @@ def test_a_norms_launch_has_fewer_than_2_32_threads(k, threads, kind):
     def norm(rows):
         return said("alofa_rmsnorm_mx", A, kind, B, 0, None, 0, 0, 0, None, 0, C, 1e-6, rows, k, 0)
     assert "than a launch takes" in norm(most + 1) and "no ROCm-capable device" in norm(most)
+
+
+@no_gpu
+@pytest.mark.parametrize("kind", [0, 4])
+@pytest.mark.parametrize("kernel", ["stream", "stream64x64", "64x64"])
+@pytest.mark.parametrize("M", [1, 20, 70])
+def test_the_streaming_kernels_grid_has_room_for_65535_shares(M, kernel, kind):
+    def product(shares):
+        return said("alofa_gemm_mx", None, ops.F32, 5, shares, A, B, kind, C, None, M, 5, 1 << 24, ops.STORE, ops.MX_FORMS[kernel], 0)
+    assert "no ROCm-capable device" in product(65535)
+    assert ("no ROCm-capable device" if kernel == "64x64" else "more shares than") in product(65536)
