@@ -3,7 +3,7 @@
 //
 // A block's scale is the smallest power of two under which its largest magnitude lies at most half a step beyond the largest element (7 for e2m1, 464
 // for e4m3), so that no element is further from its number than half a step of the elements there; never below 2^-127. Elements are rounded to the
-// nearest, ties to the even one. A block with an infinity or a NaN has the scale 255.
+// nearest, ties to the even one. A block with an infinity or a NaN has the scale 255, as has one whose scale would lie beyond 2^127 (the norm's rows alone can have numbers that large).
 //
 // They lie in the order in which the matrix cores take them, so that a wavefront's operand is one run of memory. Tiles of 16 rows by 128 numbers follow one another
 // along the row; a tile is units of 16 bytes, [group][row of 16]: of e2m1 4 groups of 32 numbers (two to a byte, the first in the low half), of e4m3 8 groups of 16.

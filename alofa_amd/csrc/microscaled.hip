@@ -21,15 +21,20 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int c0, int k, 
   }
 }
 
-// Eight numbers of a block whose three other eights are in the neighbouring lanes, to memory
-template <int kKind>
-__device__ __forceinline__ void put8(uint8_t* __restrict__ out, int64_t scales_at, int64_t r, int c, int k_tiles, const float (&v)[8]) {
+// The largest magnitude of a block, of which a lane has eight numbers and its neighbours the three other eights
+__device__ __forceinline__ uint32_t block_top(const float (&v)[8]) {
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = max(top, mx_magnitude(v[e]));
-  const uint32_t code = mx_scale_of<kKind>(quad_max(top));
+  return quad_max(top);
+}
+// Those eight numbers times 2^kUp to memory, under the scale that its largest magnitude asks for: beyond the scales' range NaN
+template <int kKind, int kUp = 0>
+__device__ __forceinline__ void put8(uint8_t* __restrict__ out, int64_t scales_at, int64_t r, int c, int k_tiles, const float (&v)[8], uint32_t top) {
+  uint32_t code = mx_scale_of<kKind>(top);
   uint32_t q[2];
   mx_pack8<kKind>(v, code, q);
+  if constexpr (kUp != 0) code = min(code + kUp, 255u);
   uint8_t* at = out + mx_place8<kKind>(r, c, k_tiles);
   if constexpr (kKind == kE2M1) *reinterpret_cast<uint32_t*>(at) = q[0];
   else *reinterpret_cast<uint2*>(at) = make_uint2(q[0], q[1]);
@@ -58,7 +63,7 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(uint8_t* __restrict__ 
       for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) put8<kKind>(tiles, scales - tiles, 4 * wave + i, lane, kStrip, v[i]);
+  for (int i = 0; i < 4; ++i) put8<kKind>(tiles, scales - tiles, 4 * wave + i, lane, kStrip, v[i], block_top(v[i]));
   __syncthreads();
   const int64_t first = static_cast<int64_t>(row_tile) * k_tiles + strip * kStrip;
   const int there = min(kStrip, k_tiles - strip * kStrip);
@@ -141,7 +146,7 @@ __global__ void __launch_bounds__(256) mx_from_codes_kernel(uint8_t* __restrict_
 }
 
 // ---- the norm between two sub-layers -------------------------------------------
-// y rounded to 24 bits so that a later rounding to fewer (22 at most) is the rounding of y itself: towards zero, and the last bit set where anything was lost
+// y rounded to 24 bits so that a later rounding to fewer (22 at most) is the rounding of y itself: towards zero, and the last bit set where anything was lost. What lies beyond the largest float comes out as that one.
 __device__ __forceinline__ float round_to_odd(double y) {
   const float f = static_cast<float>(y);
   const double d = static_cast<double>(f);
@@ -199,10 +204,19 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_mx_kernel(uint8_t* __restric
         if (8 * c + e < k) to[e] = v[e];
     }
   };
-  auto leave = [&](int c, float (&v)[8], const float (&weight)[8], double scale) {
+  auto leave = [&](int c, const float (&v)[8], const float (&weight)[8], double scale) {
+    float y[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = round_to_odd(static_cast<double>(v[e]) * scale * static_cast<double>(weight[e]));
-    put8<kKind>(out, scales_at, r, c, k_tiles, v);
+    for (int e = 0; e < 8; ++e) y[e] = round_to_odd(static_cast<double>(v[e]) * scale * static_cast<double>(weight[e]));
+    const uint32_t top = block_top(y);
+    if (top != 0x7f7fffffu) {
+      put8<kKind>(out, scales_at, r, c, k_tiles, y, top);
+      return;
+    }
+    // a y beyond the largest float (the scales go on to 464 times 2^127): the block again, divided by 2^16 (what that takes from small numbers is far below the block's elements)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = round_to_odd(static_cast<double>(v[e]) * (scale * 0x1p-16) * static_cast<double>(weight[e]));
+    put8<kKind, 16>(out, scales_at, r, c, k_tiles, y, block_top(y));
   };
   double ss = 0;
   if constexpr (kStay) {

@@ -2940,7 +2940,7 @@ def mx_from_codes(codes: torch.Tensor, scales: torch.Tensor, k: int, kind: str =
 def rmsnorm_mx(out: MXRows, x: torch.Tensor, w: torch.Tensor, eps: float, add: Optional[torch.Tensor] = None, total: Optional[torch.Tensor] = None) -> None:
     """out = rmsnorm(total) * w as microscaled rows, total = x + (add[0] + add[1] + ..) added in float32 in that order. ``x`` [T, h] float32; ``add`` [T, h] or [shares, T, h] float32 (a product's sum, or
     the shares of one: ``gemm_mx_shares``); ``total`` [T, h] float32 receives the sum and may be ``x`` itself (no other overlap); it goes with ``add``. The squares' sum and the scaling are in float64, so that a row's elements do
-    not depend on anything but the row."""
+    not depend on anything but the row. Numbers beyond the largest float32 have their own elements as far as scales go (7 or 464 times 2^127); behind that their block is NaN."""
     if type(out) is MXRows and eps > 0 and _here() == out.device and (sizes := _native().mx_norm(x, w, add, total, out.rows, out.k, out.device)) is not None:
         ldx, shares, stride, ld_add, ld_total = sizes
         _call("alofa_rmsnorm_mx", out.buffer, out.number, x, ldx, add, shares, stride, ld_add, total, ld_total, w, _F(eps), out.rows, out.k, _stream_on(out.device))

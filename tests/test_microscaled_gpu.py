@@ -540,3 +540,27 @@ def test_every_kernel_takes_shares(M, N, K, shares, kind, kernel):
     for s in range(shares):
         cut = slice(128 * (tiles * s // shares), 128 * (tiles * (s + 1) // shares))
         assert (np.abs(got[s] - av[:, cut] @ wv[:, cut].T) <= off_by(av[:, cut], wv[:, cut])).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("k", [96, 896, 2500, 9000])
+def test_norm_beyond_the_largest_float(k, kind):
+    """Weights so large that rows come out beyond 2^128: elements of their own as far as scales go, NaN behind that. Read by a product with 2^-20 times the identity, whose outputs fit a float."""
+    x, w = numbers(6, k, 21, 0), numbers(1, k, 22, 0)[0]
+    x[1, 1:], x[2, 2:], x[5] = 0, 0, 0      # (a number alone in its row: the root of k times its weight)
+    w[:40] *= np.float32(1e38)
+    w[:3] = 3e38, -3e38, 2.0 ** 100
+    w[64:70] = 3.4028235e38, 1e-38, -1.0, 3.4e38, 1e34, 0.0
+    y = pm.norm(x.astype(np.float64), w.astype(np.float64), 1e-6)
+    assert (np.abs(y) >= 2.0 ** 128).any()
+    want = pm.rounded(y, kind)
+    q = ops.MXRows(6, k, kind, DEV)
+    q.buffer.fill_(255)
+    ops.rmsnorm_mx(q, on(x), on(w), 1e-6)
+    out = torch.empty(6, k, device=DEV)
+    ops.gemm_mx(out, q, made(np.eye(k, dtype=np.float32) * np.float32(2.0 ** -20), "e2m1"))
+    got, bad = out.double().cpu().numpy(), np.isnan(want).any(1)
+    assert not bad.all() and np.isnan(got[bad]).all()      # (a NaN takes its row of the product along)
+    same(got[~bad], want[~bad] * 2.0 ** -20)
+    with np.errstate(over="ignore"):      # (beyond 2^128 a float is infinite)
+        same(read(q), want.astype(np.float32).astype(np.float64))
