@@ -319,6 +319,12 @@ extern "C" int alofa_gemm_mx(void* out, int dtype, int64_t ldo, int shares, floa
   const int k_tiles = static_cast<int>(mx_tiles(K, 128));
   ALOFA_REQUIRE(shares >= 1 && shares <= k_tiles && (out == nullptr || (shares > 1) == (parts != nullptr)) && reinterpret_cast<uintptr_t>(parts) % 16 == 0, "gemm_mx: shares=%d K=%lld", shares, static_cast<long long>(K));
   ALOFA_REQUIRE(form >= -1 && form < kMxForms, "gemm_mx: form=%d", form);
+  {
+    const MxPlace read[] = {MxPlace::held(a, M, K, a_kind), MxPlace::held(w, N, K, kE2M1), MxPlace::run(bias, 4 * N)}, to = MxPlace::numbers(out, ldo, M, N, dtype == kF32 ? 4 : 2), sums = MxPlace::run(parts, shares * M * N * 4);
+    bool meet = to.meets(sums);
+    for (const MxPlace& r : read) meet = meet || to.meets(r) || sums.meets(r);
+    ALOFA_REQUIRE(!meet, "gemm_mx: what is written overlaps what is read");
+  }
   if (form < 0) form = plan_for(M, N, k_tiles, a_kind, false, shares).form;
   auto aligned = [](const void* p, int64_t ld, int code) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % (code == kF32 ? 4 : 8) == 0; };
   const int out_vec = out && aligned(out, ldo, dtype);
@@ -338,6 +344,8 @@ extern "C" int alofa_gemm_mx(void* out, int dtype, int64_t ldo, int shares, floa
 extern "C" int alofa_gemm_swiglu_mx(void* out, int out_kind, const void* a, int a_kind, const void* gate, const void* up, int64_t M, int64_t N, int64_t K, int gelu, int form, hipStream_t stream) {
   if (!product_fits("gemm_swiglu_mx", a, a_kind, gate, M, N, K) || !product_fits("gemm_swiglu_mx", a, a_kind, up, M, N, K)) return 1;
   ALOFA_REQUIRE(out && reinterpret_cast<uintptr_t>(out) % 16 == 0 && (out_kind == kE2M1 || out_kind == kE4M3), "gemm_swiglu_mx: output does not fit: kind=%d", out_kind);
+  const MxPlace held = MxPlace::held(out, M, N, out_kind);
+  ALOFA_REQUIRE(!held.meets(MxPlace::held(a, M, K, a_kind)) && !held.meets(MxPlace::held(gate, N, K, kE2M1)) && !held.meets(MxPlace::held(up, N, K, kE2M1)), "gemm_swiglu_mx: what is written overlaps what is read");
   const int k_tiles = static_cast<int>(mx_tiles(K, 128)), out_tiles = static_cast<int>(mx_tiles(N, 128));
   const MxMatrix ma = matrix_of(a, M, K, a_kind), mg = matrix_of(gate, N, K, kE2M1), mu = matrix_of(up, N, K, kE2M1);
   const int64_t at = mx_scales_at(M, N, out_kind);

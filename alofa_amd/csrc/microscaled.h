@@ -22,6 +22,26 @@ __host__ __device__ constexpr int mx_units(int kind) { return kind == kE2M1 ? 64
 // where the scales begin, in bytes
 __host__ __device__ constexpr int64_t mx_scales_at(int64_t rows, int64_t k, int kind) { return mx_tiles(rows, 16) * mx_tiles(k, 128) * mx_units(kind) * 16; }
 
+__host__ constexpr int64_t mx_bytes(int64_t rows, int64_t k, int kind) { return mx_scales_at(rows, k, kind) + mx_tiles(rows, 16) * mx_tiles(k, 128) * 64; }
+
+// Where an operand lies: so many rows of so many bytes, ld bytes apart; microscaled rows are one run. Blocks write while others still read, so what is written may not meet what is read.
+struct MxPlace {
+  uintptr_t at;
+  int64_t ld, rows, bytes;
+  static MxPlace run(const void* p, int64_t bytes) { return {reinterpret_cast<uintptr_t>(p), bytes, 1, bytes}; }
+  static MxPlace held(const void* p, int64_t rows, int64_t k, int kind) { return run(p, mx_bytes(rows, k, kind)); }
+  static MxPlace numbers(const void* p, int64_t ld, int64_t rows, int64_t k, int size) { return {reinterpret_cast<uintptr_t>(p), ld * size, rows, k * size}; }
+  uintptr_t end() const { return at + (rows - 1) * ld + bytes; }
+  // (columns side by side in the same rows do not meet; rows of different lengths that lie between each other are taken to)
+  bool meets(const MxPlace& o) const {
+    if (at == 0 || o.at == 0 || at >= o.end() || o.at >= end()) return false;
+    const int64_t step = rows > 1 ? ld : o.ld;
+    if ((rows > 1 && o.rows > 1 && ld != o.ld) || step < bytes || step < o.bytes) return true;
+    const int64_t apart = o.at >= at ? static_cast<int64_t>((o.at - at) % step) : (step - static_cast<int64_t>((at - o.at) % step)) % step;
+    return apart < bytes || apart + o.bytes > step;
+  }
+};
+
 // The scale byte of a block whose largest magnitude has these bits (infinities and NaN included: their bits are the largest)
 template <int kKind>
 __device__ __forceinline__ uint32_t mx_scale_of(uint32_t top) {

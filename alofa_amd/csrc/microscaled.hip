@@ -267,6 +267,7 @@ using namespace alofa;
 extern "C" int alofa_mx_quantize(void* out, int kind, const void* x, int dtype, int64_t ldx, int64_t rows, int64_t k, hipStream_t stream) {
   if (!sizes_fit("mx_quantize", kind, rows, k)) return 1;
   ALOFA_REQUIRE(out && x && aligned16(out) && (dtype == kF32 || dtype == kBF16) && ldx >= 0, "mx_quantize: operands do not fit: dtype=%d ldx=%lld", dtype, static_cast<long long>(ldx));
+  ALOFA_REQUIRE(!MxPlace::held(out, rows, k, kind).meets(MxPlace::numbers(x, ldx, rows, k, dtype == kF32 ? 4 : 2)), "mx_quantize: what is written overlaps what is read");
   const int k_tiles = static_cast<int>(mx_tiles(k, 128));
   const int64_t at = mx_scales_at(rows, k, kind);
   const int strips = (k_tiles + kStrip - 1) / kStrip;
@@ -285,6 +286,7 @@ extern "C" int alofa_mx_quantize(void* out, int kind, const void* x, int dtype, 
 extern "C" int alofa_mx_values(void* out, int dtype, int64_t ldo, const void* q, int kind, int64_t rows, int64_t k, hipStream_t stream) {
   if (!sizes_fit("mx_values", kind, rows, k)) return 1;
   ALOFA_REQUIRE(out && q && aligned16(q) && (dtype == kF32 || dtype == kBF16) && ldo >= 0, "mx_values: operands do not fit: dtype=%d ldo=%lld", dtype, static_cast<long long>(ldo));
+  ALOFA_REQUIRE(!MxPlace::held(q, rows, k, kind).meets(MxPlace::numbers(out, ldo, rows, k, dtype == kF32 ? 4 : 2)), "mx_values: what is written overlaps what is read");
   const int k_tiles = static_cast<int>(mx_tiles(k, 128)), strips = (k_tiles + kStrip - 1) / kStrip;
   const int64_t at = mx_scales_at(rows, k, kind);
   const unsigned blocks = static_cast<unsigned>(mx_tiles(rows, 16) * strips);
@@ -302,6 +304,9 @@ extern "C" int alofa_mx_values(void* out, int dtype, int64_t ldo, const void* q,
 extern "C" int alofa_mx_from_codes(void* out, int kind, const void* codes, int64_t ld_codes, const void* scales, int64_t ld_scales, int64_t rows, int64_t k, hipStream_t stream) {
   if (!sizes_fit("mx_from_codes", kind, rows, k)) return 1;
   ALOFA_REQUIRE(out && codes && scales && aligned16(out) && ld_codes >= 0 && ld_scales >= 0, "mx_from_codes: operands do not fit");
+  const MxPlace held = MxPlace::held(out, rows, k, kind);
+  ALOFA_REQUIRE(!held.meets(MxPlace::numbers(codes, ld_codes, rows, kind == kE2M1 ? mx_tiles(k, 2) : k, 1)) && !held.meets(MxPlace::numbers(scales, ld_scales, rows, mx_tiles(k, 32), 1)),
+                "mx_from_codes: what is written overlaps what is read");
   const int k_tiles = static_cast<int>(mx_tiles(k, 128));
   const int64_t at = mx_scales_at(rows, k, kind);
   const unsigned blocks = static_cast<unsigned>(mx_tiles(rows * 16 * k_tiles, 256));
@@ -317,6 +322,15 @@ extern "C" int alofa_rmsnorm_mx(void* out, int kind, const float* x, int64_t ldx
   if (!sizes_fit("rmsnorm_mx", kind, rows, k)) return 1;
   ALOFA_REQUIRE(out && x && w && aligned16(out) && shares >= 0 && (shares == 0 || add) && (shares == 0 || total) && ldx >= 0 && ld_add >= 0 && share_stride >= 0 && ld_total >= 0 && eps > 0.f,
                 "rmsnorm_mx: operands do not fit: shares=%d eps=%g", shares, static_cast<double>(eps));
+  {
+    const MxPlace held = MxPlace::held(out, rows, k, kind), from = MxPlace::numbers(x, ldx, rows, k, 4), sum = MxPlace::numbers(total, ld_total, rows, k, 4), weights = MxPlace::run(w, 4 * k);
+    bool meet = held.meets(from) || held.meets(sum) || held.meets(weights) || sum.meets(weights) || ((total != x || (rows > 1 && ld_total != ldx)) && sum.meets(from));
+    for (int s = 0; s < shares; ++s) {
+      const MxPlace share = MxPlace::numbers(add + s * share_stride, ld_add, rows, k, 4);
+      meet = meet || held.meets(share) || sum.meets(share);
+    }
+    ALOFA_REQUIRE(!meet, "rmsnorm_mx: what is written overlaps what is read (the sum may take the place of x itself)");
+  }
   const int k_tiles = static_cast<int>(mx_tiles(k, 128)), n = static_cast<int>(k), units = 16 * k_tiles;
   const int threads = units <= 256 ? 256 : units <= 512 ? 512 : units <= 768 ? 768 : units <= 1024 ? 1024 : 256;
   ALOFA_REQUIRE(rows * threads < INT64_C(1) << 32, "rmsnorm_mx: more rows than a launch takes: %lld of %lld numbers", static_cast<long long>(rows), static_cast<long long>(k));

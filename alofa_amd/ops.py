@@ -2827,7 +2827,8 @@ class MXRows:
     """``rows`` x ``k`` numbers in blocks of 32 along a row: elements of 4 bits (``kind`` "e2m1") or 8 ("e4m3") times a power of two per block, in the order in which the
     matrix cores take them (csrc/microscaled.h). A matrix [out_features, in_features] that a product reads is such rows of "e2m1". ``buffer``: contiguous uint8 on the
     GPU of at least ``MXRows.bytes(rows, k, kind)``, 16-byte aligned, that they are to lie in; without it, it is allocated. What it holds is made by ``mx_quantize``,
-    ``mx_from_codes``, ``rmsnorm_mx`` or ``gemm_swiglu_mx``; rows' places follow from all three sizes, so that a buffer is read as what it was made as."""
+    ``mx_from_codes``, ``rmsnorm_mx`` or ``gemm_swiglu_mx``; rows' places follow from all three sizes, so that a buffer is read as what it was made as. None of the operators below works in place:
+    what they write may not overlap what they read, but for ``total`` of ``rmsnorm_mx``."""
     __slots__ = ("rows", "k", "kind", "buffer", "number", "device")      # (number: the kind's, as csrc/microscaled.h has it; device: its index)
 
     def __init__(self, rows: int, k: int, kind: str, device=None, buffer: Optional[torch.Tensor] = None):

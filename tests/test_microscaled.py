@@ -139,3 +139,44 @@ def test_the_streaming_kernels_grid_has_room_for_65535_shares(M, kernel, kind):
         return said("alofa_gemm_mx", None, ops.F32, 5, shares, A, B, kind, C, None, M, 5, 1 << 24, ops.STORE, ops.MX_FORMS[kernel], 0)
     assert "no ROCm-capable device" in product(65535)
     assert ("no ROCm-capable device" if kernel == "64x64" else "more shares than") in product(65536)
+
+
+NO_GPU, MEETS = "no ROCm-capable device", "what is written overlaps what is read"
+
+
+@no_gpu
+@pytest.mark.parametrize("kind", ["e2m1", "e4m3"])
+def test_what_is_written_may_not_overlap_what_is_read(kind):
+    number = ops.MX_KINDS[kind]
+    rows, k, n = 40, 256, 256      # (N = K: gated rows would fit the place of the rows they are made of)
+    held, matrix = ops.MXRows.bytes(rows, k, kind), ops.MXRows.bytes(n, k, "e2m1")
+
+    def quantise(out, x, ldx=k, dtype=ops.F32):
+        return said("alofa_mx_quantize", out, number, x, dtype, ldx, rows, k, 0)
+
+    def values(out, q, ldo=k):
+        return said("alofa_mx_values", out, ops.F32, ldo, q, number, rows, k, 0)
+
+    def codes(out, codes, scales):
+        return said("alofa_mx_from_codes", out, number, codes, k, scales, k // 32, rows, k, 0)
+
+    def norm(out, x, w, add, total, ldx=k, ld_add=k, ld_total=k, shares=2, stride=rows * k):
+        return said("alofa_rmsnorm_mx", out, number, x, ldx, add, shares, stride, ld_add, total, ld_total, w, 1e-6, rows, k, 0)
+
+    def product(out, a, w, bias=None, parts=None, shares=1):
+        return said("alofa_gemm_mx", out, ops.F32, n, shares, parts, a, number, w, bias, rows, n, k, ops.STORE, -1, 0)
+
+    def gated(out, a, gate, up):
+        return said("alofa_gemm_swiglu_mx", out, number, a, number, gate, up, rows, n, k, 0, -1, 0)
+    apart = [quantise(A, B), quantise(A, A + held), quantise(A + rows * k * 4, A), quantise(A + 4 * k, A, 4096),      # (the last two: behind all rows, and in the room between two of them)
+             values(A, B), codes(A, B, C), norm(A, B, C, D, B), norm(A, B, C, D, D + 8 * rows * k), norm(A, B, C, D, B + 4 * k, 2 * k, k, 2 * k), norm(A, B, C, B, B + 8 * rows * k), norm(A, B, C, 0, 0, shares=0),
+             product(A, B, C), product(A, B, C, D), product(A, B, C, None, D, 2), product(A, A + 4 * rows * n, C), gated(A, B, C, D), gated(A, B, C, C), gated(A, A + held, C, D)]
+    meet = [quantise(A, A), quantise(A + 64, A, 4096), quantise(A, A + held - 16), quantise(A + rows * k * 4 - 16, A), values(A, A), values(A + held - 4, A), codes(A, A, B), codes(A, B, A + 16), codes(A, A + held - 1, B),
+            norm(A, A, B, C, C + 8 * rows * k), norm(A, B, C, D, A), norm(A, B, A, C, D), norm(A, B, C, D, D), norm(A, B, C, D, D + 4 * rows * k), norm(A, B, C, A + 16, D), norm(A, B, C, D, C + 16 - 4 * k),
+            norm(A, B, C, D, B + 4), norm(A, B, C, D, B + 4 * k, 2 * k, k, 3 * k), norm(A, B, C, D, B, 0), norm(A, B, C, D, B + 4 * k - 16, 2 * k, k, 2 * k), norm(A, A, B, 0, 0, shares=0),
+            product(A, A, C), product(A, B, A), product(A, B, C, A), product(A, B, C, None, A, 2), product(A, B, C, None, B, 2), product(None, B, C, None, C + matrix - 16, 2), product(A + held - 4, A, C),
+            gated(A, A, B, C), gated(A, B, A, C), gated(A, B, C, A), gated(A + held - 16, A, B, C), gated(A, B, A + held - 16, C), gated(A + matrix - 16, B, C, A)]
+    for i, s in enumerate(apart):
+        assert NO_GPU in s, (i, s)
+    for i, s in enumerate(meet):
+        assert MEETS in s, (i, s)

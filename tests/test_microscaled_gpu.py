@@ -564,3 +564,24 @@ def test_norm_beyond_the_largest_float(k, kind):
     same(got[~bad], want[~bad] * 2.0 ** -20)
     with np.errstate(over="ignore"):      # (beyond 2^128 a float is infinite)
         same(read(q), want.astype(np.float32).astype(np.float64))
+
+
+def test_gated_products_in_the_place_of_their_rows_are_refused():
+    a, w = made(numbers(40, 64, 1), "e4m3"), made(numbers(64, 64, 2), "e2m1")
+    before = a.buffer.clone()
+    for out in (a, ops.MXRows(40, 64, "e4m3", buffer=a.buffer), ops.MXRows(40, 64, "e2m1", buffer=a.buffer[1024:])):
+        with pytest.raises(AlofaError, match="overlaps"):
+            ops.gemm_swiglu_mx(out, a, w, w)
+    torch.cuda.synchronize()
+    assert torch.equal(a.buffer, before)
+
+
+def test_the_sum_in_columns_beside_the_stream():
+    wide = on(numbers(40, 512, 1, 1))
+    x, w, add = wide[:, :256], on(numbers(1, 256, 2, 1)[0]), on(numbers(40, 256, 3, 1))
+    q, r, total = ops.MXRows(40, 256, "e4m3", DEV), ops.MXRows(40, 256, "e4m3", DEV), wide[:, 256:]
+    want, stream = torch.empty(40, 256, device=DEV), x.clone()
+    ops.rmsnorm_mx(q, x, w, 1e-6, add=add, total=want)
+    ops.rmsnorm_mx(r, x, w, 1e-6, add=add, total=total)
+    assert torch.equal(total, want) and torch.equal(x, stream)
+    same(read(r), read(q))
