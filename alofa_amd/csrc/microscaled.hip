@@ -50,8 +50,7 @@ constexpr int kStrip = 4;      // tiles along a row that a block takes
 template <typename T, int kKind, bool kVec>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(uint8_t* __restrict__ out, int64_t scales_at, const T* __restrict__ x, int64_t ldx, int rows, int k, int k_tiles, int strips) {
   constexpr int kTile = mx_units(kKind) * 16;
-  __shared__ __attribute__((aligned(16))) uint8_t tiles[kStrip * kTile];
-  __shared__ __attribute__((aligned(16))) uint8_t scales[kStrip * 64];
+  __shared__ __attribute__((aligned(16))) uint8_t tiles[kStrip * (kTile + 64)];      // ... and their scales behind them, as in memory
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, row_tile = blockIdx.x / strips, strip = blockIdx.x % strips, c = strip * kStrip * 16 + lane;
   float v[4][8];
 #pragma unroll
@@ -63,12 +62,12 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(uint8_t* __restrict__ 
       for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) put8<kKind>(tiles, scales - tiles, 4 * wave + i, lane, kStrip, v[i], block_top(v[i]));
+  for (int i = 0; i < 4; ++i) put8<kKind>(tiles, kStrip * kTile, 4 * wave + i, lane, kStrip, v[i], block_top(v[i]));
   __syncthreads();
   const int64_t first = static_cast<int64_t>(row_tile) * k_tiles + strip * kStrip;
   const int there = min(kStrip, k_tiles - strip * kStrip);
   for (int i = threadIdx.x; i < there * (kTile / 16); i += 256) reinterpret_cast<uint4*>(out + first * kTile)[i] = reinterpret_cast<const uint4*>(tiles)[i];
-  if (static_cast<int>(threadIdx.x) < there * 4) reinterpret_cast<uint4*>(out + scales_at + first * 64)[threadIdx.x] = reinterpret_cast<const uint4*>(scales)[threadIdx.x];
+  if (static_cast<int>(threadIdx.x) < there * 4) reinterpret_cast<uint4*>(out + scales_at + first * 64)[threadIdx.x] = reinterpret_cast<const uint4*>(tiles + kStrip * kTile)[threadIdx.x];
 }
 
 __device__ __forceinline__ float mx_scaled(float element, uint32_t code) { return code == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(element, static_cast<int>(code) - 127); }
