@@ -1,4 +1,6 @@
 """Microscaled rows on the GPU: every operator against plain numpy in 64 bits, at the sizes, values and layouts where it could go wrong."""
+import functools
+
 import numpy as np
 import pytest
 import torch
@@ -585,3 +587,72 @@ def test_the_sum_in_columns_beside_the_stream():
     ops.rmsnorm_mx(r, x, w, 1e-6, add=add, total=total)
     assert torch.equal(total, want) and torch.equal(x, stream)
     same(read(r), read(q))
+
+
+SHARED_OUT = [(40, 97, 8192, "e4m3"), (20, 64, 9001, "e4m3"), (300, 66, 8200, "e4m3")] + [(*s, kind) for kind in KINDS for s in ((1, 7, 40000), (5, 33, 40000), (33, 131, 16385), (130, 50, 12000), (64, 96, 16384))]
+
+
+@pytest.mark.parametrize("M,N,K,kind", SHARED_OUT)
+def test_products_whose_sum_the_rule_shares_out(M, N, K, kind):
+    """Shares of K that a launch of its own adds up, with every epilogue."""
+    shares = ops._answer("alofa_gemm_mx_shares", M, N, K, ops.MX_KINDS[kind], 0)
+    assert shares > 1
+    a, w, av, wv = operands(M, N, K, kind, M + N + K)
+    want, off = av @ wv.T, off_by(av, wv)
+    bias, old = numbers(1, N, 3, 3)[0], numbers(M, N, 4, 3)
+    asked = []
+
+    def scratch(name, shape, dtype):
+        asked.append(shape)
+        return torch.full(shape, float("nan"), dtype=dtype, device=DEV)
+    for by in (0, 8, 3):
+        for dtype in (torch.float32, torch.bfloat16):
+            step = 2.0 ** -24 if dtype is torch.float32 else 2.0 ** -8
+            for b in (None, bias):
+                out = strided(old, dtype, by)
+                ops.gemm_mx(out, a, w, None if b is None else on(b), scratch=scratch)
+                ref = want if b is None else want + b
+                assert (np.abs(out.double().cpu().numpy() - ref) <= off + 2.0 ** -23 * np.abs(ref) + step * (np.abs(ref) + off)).all()
+                assert by == 0 or (out._base[:, N:] == 7).all()
+        out = strided(old, torch.float32, by)
+        ops.gemm_mx(out, a, w, add_to_out=True)
+        ref = want + old
+        assert (np.abs(out.double().cpu().numpy() - ref) <= off + 2.0 ** -24 * (np.abs(ref) + off)).all()
+        assert by == 0 or (out._base[:, N:] == 7).all()
+    assert asked == [(shares * M * N,)] * 12
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,k,shares", [(1, 40, 2), (5, 896, 3), (17, 2176, 2), (6, 1000, 4), (3, 9000, 2)])
+def test_norm_of_shares_and_rows_that_lie_apart_or_are_one_and_the_same(rows, k, shares, kind):
+    """Shares in wider rows, at distances of their own, one share or one row many times over; a weight and a stream at any address."""
+    x, w = numbers(rows, k, 5, 2), numbers(1, k, 6, 0)[0]
+    add = np.stack([numbers(rows, k, 7 + s, 2) for s in range(shares)])
+
+    def check(xd, wd, parts, xv=x, addv=add):
+        total = xv + functools.reduce(np.add, addv)
+        q, t = ops.MXRows(rows, k, kind, DEV), torch.empty(rows, k, device=DEV)
+        q.buffer.fill_(255)
+        ops.rmsnorm_mx(q, xd, wd, 1e-6, add=parts, total=t)
+        same(t.double().cpu().numpy(), total.astype(np.float64))
+        same(read(q), pm.rounded(pm.norm(total.astype(np.float64), w.astype(np.float64), 1e-6), kind))
+    xd, wd, ad = on(x), on(w), on(add)
+    for rows_by, k_by in ((0, 8), (2, 0), (3, 4), (1, 3)):      # (rows and columns between the shares)
+        room = torch.full((shares, rows + rows_by, k + k_by), float("nan"), device=DEV)
+        room[:, :rows, :k] = ad
+        check(xd, wd, room[:, :rows, :k])
+    by_row = torch.full((rows, shares, k), float("nan"), device=DEV)      # (the shares of a row side by side)
+    by_row.copy_(ad.transpose(0, 1))
+    check(xd, wd, by_row.transpose(0, 1))
+    check(xd, wd, ad[:1].expand(shares, rows, k), addv=add[:1].repeat(shares, 0))
+    check(xd, wd, ad[:, :1].expand(shares, rows, k), addv=add[:, :1].repeat(rows, 1))
+    check(xd, wd, ad[0].expand(shares, rows, k), addv=add[:1].repeat(shares, 0))
+    check(xd[:1].expand(rows, k), wd, ad, xv=x[:1].repeat(rows, 0))
+    check(xd, wd, xd.expand(shares, rows, k), addv=x[None].repeat(shares, 0))      # (what is added may be the stream)
+    odd = torch.empty(k + 1, device=DEV)[1:]
+    odd.copy_(wd)
+    assert odd.data_ptr() % 16 == 4
+    check(xd, odd, ad)
+    at = torch.empty(rows * k + 1, device=DEV)[1:].view(rows, k)
+    at.copy_(xd)
+    check(at, wd, ad)
