@@ -148,3 +148,50 @@ def test_shares_of_the_product_down_go_to_the_next_layers_norm(tmp_path):
     assert_close(collect(replayer, whole("w", ids))["w"], ref, "bfloat16", "whole")
     assert_close(collect(replayer, portions("p", ids, (40, 17, 23, 10)))["p"], ref, "bfloat16", "portions")
     assert_close(collect(replayer, bulk_and_tail("b", ids, 84))["b"], ref, "bfloat16", "bulk then one by one")
+
+
+@pytest.mark.parametrize("T", [1, 23, 90])
+def test_a_layer_whose_output_product_has_a_bias(T):
+    """Layers of any registered design may have one. With a feed-forward that adds nothing the layer with it is the layer without it and the bias; and its second half reads that sum."""
+    from alofa_amd import ops
+    from alofa_amd.cache import CacheManager
+    from alofa_amd.config import LayerSpec, ModelSpec, PartSpec, RunEntry
+    from alofa_amd.engine import StepEntry, StepFunction
+    from alofa_amd.model import Model, expected_tensors, runtime
+    from alofa_amd.parts.microscaled import microscaled
+    from alofa_amd.weights import random_tensors
+    h, H, kv, d, inter, V = 160, 4, 2, 32, 352, 50
+    rng = np.random.default_rng(T)
+    stream = rng.standard_normal((T, h)).astype(np.float32)
+
+    def run(bias, weights):
+        layer = LayerSpec("l.", PartSpec("prenorm"), dict(
+            mixer=PartSpec("gqa_attention", {"prefix": "l.att.", "hidden": h, "heads": H, "kv_heads": kv, "head_dim": d, "qkv_bias": True, "out_bias": bias, "window": None,
+                                             "position": PartSpec("none", {"head_dim": d})}),
+            feed_forward=PartSpec("swiglu", {"prefix": "l.ff.", "hidden": h, "intermediate": inter}),
+            norms=(PartSpec("rmsnorm", {"name": "l.n0", "width": h, "eps": 1e-6}), PartSpec("rmsnorm", {"name": "l.n1", "width": h, "eps": 1e-6}))))
+        spec = microscaled(ModelSpec(h, V, 128, PartSpec("token_embedding", {"name": "emb", "vocab": V, "width": h}), (layer,), (RunEntry(0),),
+                                     PartSpec("rmsnorm", {"name": "nf", "width": h, "eps": 1e-6}), PartSpec("lm_head", {"name": "head", "tied_to": "emb", "vocab": V, "width": h})))
+        expected = expected_tensors(spec)
+        weights = weights or random_tensors(expected, 6, std=0.3, store_dtype="float32")
+        model = Model(spec, {n: weights[n] for n in expected if n in weights}, runtime("bfloat16"))
+        fn = StepFunction(model, CacheManager(model.cache_needs(), model.state_needs(), 8, 16, 2, device=model.rt.device, dtype=torch.bfloat16), 128)
+        fn.cache.admit(0)
+        ctx, _, _ = fn.begin([StepEntry(0, [1] * T, [])])
+        out = torch.from_numpy(stream).cuda()
+        model.blocks[0].forward(ctx, 0, out)
+        return out.cpu().numpy(), weights
+    got, weights = run(True, None)
+    assert weights["l.att.o_proj.bias"].abs().max() > 0.1
+    idle = dict(weights, **{"l.ff.down_proj.weight": torch.zeros(h, inter)})
+    without, mixed_in = run(False, idle)[0], run(True, idle)[0]
+    bias = weights["l.att.o_proj.bias"].numpy()
+    # (one sum is rounded twice on the way, the other three times, half a unit of what is there each; the products themselves are the same up to the order of a sum of 128 numbers in shares of one)
+    assert np.abs(mixed_in - (without + bias)).max() <= 8 * 2.0 ** -24 * (np.abs(without) + np.abs(bias) + np.abs(mixed_in) + np.abs(stream)).max()
+    f64 = {n: t.double().numpy() for n, t in weights.items()}
+    t = mixed_in.astype(np.float64)
+    n = px.rounded(px.norm(t, f64["l.n1"], 1e-6), "e4m3")
+    gate, up, down = (px.rounded(f64[f"l.ff.{m}_proj.weight"], "e2m1") for m in ("gate", "up", "down"))
+    want = t + px.rounded(px.silu(n @ gate.T) * (n @ up.T), "e4m3") @ down.T
+    # (an element here and there goes to its neighbour by a last bit: were a part in 256 of them all a whole step off)
+    assert np.linalg.norm(got - want) / np.linalg.norm(want) <= 2.0 ** -24 + 2.0 ** -8
