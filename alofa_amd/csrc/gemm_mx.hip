@@ -49,10 +49,10 @@ struct MxOperand {
 // ---- few rows: the matrix is streamed once -------------------------------------
 // A block computes NT tiles of 16 outputs for MT tiles of 16 rows. Its waves share out K tile by tile, every wave with the next tile of the matrix on its way under the products of one; the waves' sums meet in LDS and are
 // added in the waves' order. Nothing is waited for together but at the end. Lanes whose row lies behind the last one read the last one again: memory is asked for rows that there are only.
-// Up to 16 rows memory bounds it: gate and up of 18,944 x 3,584 take 16.6 us (4.3 TB/s; 27,648 x 5,120 30.7, 4.9), 3,584 x 18,944 11.3, 7,168 x 5,120 6.6. What keeps it busy is waves side by side, not tiles ahead: with
+// Up to 16 rows memory bounds it: gate and up of 18,944 x 3,584 take 16.9 us (4.3 TB/s; 27,648 x 5,120 30.8, 4.9), 3,584 x 18,944 8.5 (4.3), 7,168 x 5,120 6.1. What keeps it busy is waves side by side, not tiles ahead: with
 // two and three tiles a set, whose registers leave room for fewer, 5,120 x 5,120 against 8 rows took 7.1 and 9.1 us (6.0), gate and up with eight waves a block 22.3.
-// With more rows it is what the caches give, 13 TB/s over all compute units (333 rows against 18,944 x 3,584 by 4 x 4 tiles: 622 MB in 50 us); so rows and matrix are taken by equal numbers of tiles where blocks are many. Where
-// they are few, 2 x 4 tiles and eight waves keep more compute units busy: 64 rows against 4,608 x 3,584 take 7.6 us (4 x 4: 10.1; 1 x 4: 11.0), against 18,944 x 3,584 22.1 (18.2).
+// With more rows it is what the caches give, 13 TB/s over all compute units (333 rows against 18,944 x 3,584 by 4 x 4 tiles: 622 MB in 48 to 52 us); so rows and matrix are taken by equal numbers of tiles where blocks are many. Where
+// they are few, 2 x 4 tiles and eight waves keep more compute units busy: 64 rows against 4,608 x 3,584 take 7.6 us (4 x 4: 10.1; 1 x 4: 11.0), against 18,944 x 3,584 20.8 (17.2).
 template <int kAct, int NT, int MT, int kWaves>
 __device__ __forceinline__ void mx_stream(const MxMatrix& a, const MxMatrix (&w)[NT], const int (&w_tile)[NT], int M, int first_m_tile, int k_begin, int k_end, int k_tiles, f32x4 (&acc)[NT][MT]) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, shift = 8 * (lane / 16);
@@ -137,8 +137,9 @@ __global__ void __launch_bounds__(kWaves * kWave, MT == 4 ? 2 : 3) mx_stream_ker
   }
 }
 
-// Gate and up of the same 32 outputs, act(gate) * up, one block of a microscaled row of the output. 18,944 x 3,584: 16.4 us up to 8 rows (4.4 TB/s of matrices), 17.0 at 16, 20.3 at 32, where memory waits for the products;
-// four tiles of rows would take 245 registers and 28.0 us at 64, as tiles of 64 x 64 do.
+// Gate and up of the same 32 outputs, act(gate) * up, one block of a microscaled row of the output. 18,944 x 3,584: 16.3 us up to 8 rows (4.4 TB/s of matrices), 16.9 at 16, 19.9 at 32, where memory waits for the products;
+// four tiles of rows would take 245 registers and 28.0 us at 64, as tiles of 64 x 64 do. The gate is the general form with expf and a division here; the tiles' epilogue, which has more of it to do, takes __expf and `over`, so that a
+// row's outputs by the one and by the other differ by more than the order of a sum (2^-15 of a number at most where gates are below 2^7, before it becomes an element).
 template <int kAct, int kOut, int MT, int kWaves>
 __global__ void __launch_bounds__(kWaves * kWave, MT == 2 ? 2 : 4) mx_stream_gated_kernel(uint8_t* __restrict__ out, int64_t out_scales_at, int out_tiles, MxMatrix a, MxMatrix gate, MxMatrix up, int M, int N,
                                                                          int k_tiles, int gelu) {
@@ -223,9 +224,10 @@ __global__ void __launch_bounds__(256) mx_sum_kernel(TO* __restrict__ out, int64
 }
 
 // What a product takes in each form, in us, and how it is chosen: besides + more (each - 1) + turns max(alone, each * of_each), where a compute unit has `each` blocks and a block takes `step` slabs of 128 along K in a
-// turn. Fitted to 2,400 measured products (1 to 2,048 rows, matrices of 1,152 x 896 to 18,944 x 3,584 and 3,584 x 18,944; 3 % off in the mean with e4m3, 6 % with e2m1). Read along a column: tiles of 256 x 256 pay where all
-// compute units have some, small ones and the streaming kernel where blocks are few: 333 rows against 4,608 x 3,584 take 15.5 us by 64 x 64 streamed, 16.8 and 17.8 by tiles of 64 x 64 and 64 x 128, 25.4 by 128 x 128 and 41 by
-// 256 x 128; 700 rows against 18,944 x 3,584 91, 94, 80 and 85. A sum that is shared out over K takes a launch more, which adds the shares up, unless a norm does.
+// turn. Fitted to 2,412 timings of 360 products (1 to 2,048 rows, the streaming kernel's up to 512, matrices of 1,152 x 896 to 18,944 x 3,584 and 3,584 x 18,944; 3 % off in the mean with e4m3, 6 % with e2m1).
+// Of 500 other products and gated products (1 to 2,048 rows, any widths of 300 to 27,648) the form it takes is 0.8 % slower than the quickest in the mean with e4m3 (1.24 times at worst), 2.7 % with e2m1 (1.45). Read along a column: tiles of 256 x 256 pay where all
+// compute units have some, small ones and the streaming kernel where blocks are few: 333 rows against 4,608 x 3,584 take 16.7 us by 64 x 64 streamed, 18.3 and 18.8 by tiles of 64 x 64 and 64 x 128, 25.5 by 128 x 128 and 40.8 by
+// 256 x 128; 700 rows against 18,944 x 3,584 95.8, 90.7, 89.8, 79.9 and 85.7. A sum that is shared out over K takes a launch more, which adds the shares up, unless a norm does.
 struct MxCost {
   int form, rows, columns, step;
   float alone, of_each, besides, more;
@@ -242,7 +244,7 @@ constexpr MxCost kMxStream8[] = {{kMxStream, 16, 16, 8, 0.4f, 0.4f, 4.3f, 0.f}, 
 constexpr MxCost kMxStream4[] = {{kMxStream, 16, 16, 8, 0.25f, 0.25f, 4.3f, 0.f}, {kMxStream, 32, 32, 8, 0.45f, 0.45f, 4.3f, 0.f}, {kMxStream, 64, 32, 8, 0.47f, 0.47f, 4.3f, 0.5f},
                                  {kMxStream, 16, 64, 4, 0.55f, 0.55f, 4.3f, 0.f}, {kMxStream, 32, 64, 4, 0.55f, 0.55f, 4.3f, 0.f}};
 constexpr MxCost kMxWide8 = {kMxStream64x64, 64, 64, 4, 0.87f, 0.77f, 4.3f, 1.1f}, kMxWide4 = {kMxStream64x64, 64, 64, 4, 0.45f, 0.36f, 4.3f, 1.5f};
-constexpr int kMxStreamRows = 2048;      // most rows that the streaming kernel is asked for (measured up to 1,500: what it reads again and again costs more than a slab in LDS but where the matrix is small)
+constexpr int kMxStreamRows = 2048;      // most rows that the streaming kernel is weighed for. 382 products of 513 to 2,048 rows for which the rule takes it, beside every other form: with e4m3 0.4 % slower than the quickest in the mean (1.11 times at worst; without it 15 to 45 %), with e2m1 6 %, where rows are long (20,000 numbers) 1.3 to 1.55 times
 
 struct MxPlan {
   int form, shares;

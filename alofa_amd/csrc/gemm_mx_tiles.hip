@@ -7,7 +7,7 @@
 // A block of four waves and fewer outputs than a compute unit can work on at once has two teams (KS = 2): each multiplies one half of every slab, 64 along K, and the second's sums go to the first at the end. A wave's own
 // products and arithmetic do not overlap (a turn of 357 cycles of products and one of 121 of arithmetic took 469 together), another wave's do: tiles of 64 x 64 took 13.1 us where one team took 18.9 (64 rows against
 // 4,608 x 3,584), of 128 x 128 25.4 for 27.8 (and 42.5 for 44.0, 333 rows against 18,944 x 3,584).
-// Many rows are bound by the products' rate, at which the card's power allows 4.1 to 4.3 PFLOP/s of e4m3 instructions, i.e. 2.1 of products in two passes, and 5.3 to 6.2 of e2m1: 2,048 x 8,192 x 8,192 runs at 1.6 and 3.9.
+// Many rows are bound by the products' rate, at which the card's power allows 4.1 to 4.3 PFLOP/s of e4m3 instructions, i.e. 2.1 of products in two passes, and 5.3 to 6.2 of e2m1: 2,048 x 8,192 x 8,192 runs at 1.7 and 3.9.
 //
 // Operands of the instruction, lane l: row l % 32; e2m1: the 32 numbers from 32 (l / 32) on; e4m3: the sixteen from 16 (l / 32) on and the sixteen from 32 + 16 (l / 32) on; the scale of block
 // l / 32. acc[e] holds the matrix's row 8 (e / 4) + 4 (l / 32) + e % 4 against the activations' row l % 32.

@@ -43,7 +43,8 @@ __device__ __forceinline__ void put8(uint8_t* __restrict__ out, int64_t scales_a
 
 // ---- numbers to microscaled rows and back --------------------------------------
 // A block takes 16 rows by 512 columns, four tiles: a wave has four of the rows, a lane eight numbers of each. The tiles are put together in LDS and leave as whole runs (row by row, 16 bytes of each 256 would be
-// written at a time). Memory bounds both ways: 18,944 x 3,584 of bfloat16 to and from e2m1 35.3 us, 4.9 TB/s (a copy of 4 GiB: 4.7); rows that 16-byte loads cannot read, or write, 1.8 and 1.4 TB/s. Elements are
+// written at a time). Memory bounds both ways: 18,944 x 3,584 of bfloat16 to and from e2m1 35.2 us, 4.9 TB/s (a copy of 1 GiB: 5.2, of 4: 4.8); rows that 16-byte loads cannot read, or write, go number by number, 86 and 104 us, 2.0 and 1.7 TB/s
+// (no model here has such widths). Elements are
 // rounded by the conversion instructions, once, from the number itself (a power of two as the scale loses nothing).
 constexpr int kStrip = 4;      // tiles along a row that a block takes
 
@@ -172,8 +173,8 @@ __device__ __forceinline__ void add_shares(const float* __restrict__ row, int64_
 
 // total = x + (add[0] + add[1] + ..) in float, y = total / sqrt(mean(total^2) + eps) * w in double, y to microscaled rows. A block takes a row. The squares' sum and
 // y are in double so that no element depends on the order of a sum: a value next to the middle of two elements would become one or the other.
-// Memory bounds many rows: 2,048 x 3,584 with one share 26.8 us (3.6 TB/s), 2,048 x 5,120 with two 44.8 (4.0); few are bound by one row's steps one after the other, 4.3 us at 1 x 896 and 5.4 at 64 x 5,120 with four
-// shares. A block of four rows would write 64 bytes at a time for 16: 26.1 us at 2,048 rows, but 11.6 for 8.0 at 512.
+// Memory bounds many rows: 2,048 x 3,584 with one share 26.8 us (3.6 TB/s; without shares 16.2, 2.3), 2,048 x 5,120 with two 45.0 (4.0); few are bound by one row's steps one after the other, 4.4 us at 1 x 896 and 5.6 at 64 x 5,120 with four
+// shares. Rows that 16-byte loads cannot read go number by number: 2,000 x 5,001 with one share 83. A block of four rows would write 64 bytes at a time for 16: 26.1 us at 2,048 rows, but 11.6 for 8.0 at 512.
 // kStay: a row of at most 8 kThreads numbers (8,192) stays in registers between the sum and the scaling, eight a thread; else any row, read twice. (256 threads with two and three eights took 6.5 us for 5.4 at
 // 64 x 5,120 and 27.2 for 26.8 at 2,048 x 3,584: a row's steps are shorter.)
 template <int kKind, int kThreads, bool kStay, bool kVec>

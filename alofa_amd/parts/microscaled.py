@@ -6,7 +6,10 @@ it was: the stream and all sums in float32, queries, keys and values in bfloat16
 a = stream; n0 = q8(norm0(a)); qkv = n0 Wqkv^T + b; o = q8(attention(qkv)); a += o Wo^T; n1 = q8(norm1(a)); a += q8(act(n1 Wg^T) * (n1 Wu^T)) Wd^T
 
 The output product leaves the shares of its sum and the norm behind it adds them to the stream on its way. So does the product down, where its sum is
-shared out, with the first norm of the next such layer (a launch less: 4.6 us of 106 a layer, 64 rows at 3,584 x 18,944)."""
+shared out, with the first norm of the next such layer (a launch less: 4.6 us of 106 a layer, 64 rows at 3,584 x 18,944).
+
+Unlike the stored layer this one turns queries and keys and writes the cache by a launch of their own, does not say that it may be run by making another layer's launches again (its matrices
+are no tensors), and has no decode step in one launch: at 0.5B sizes, where launches are what a step costs, it is the slower one."""
 from __future__ import annotations
 
 import dataclasses
